@@ -69,10 +69,11 @@
 extern "C" {
 #endif
 
-#define TA_ABI_VERSION 5
+#define TA_ABI_VERSION 6
 
 #define TA_DTYPE_BF16 1
 #define TA_DTYPE_F16 2
+#define TA_DTYPE_F32 3          /* ta_beam_select: logits */
 
 #define TA_OK 0
 #define TA_ERR_ARG 1          /* host: invalid argument, nothing launched */
@@ -214,6 +215,88 @@ int ta_decode_append(void* kpool, void* vpool, const void* k_new, const void* v_
                      int64_t pool_tokens, int32_t head_dim, int32_t dtype, int32_t* klen, const int32_t* tail_jobs,
                      int32_t num_tails, const int64_t* count, int32_t offset, int32_t num_jobs, int32_t* status,
                      void* stream);
+
+/*
+ * One layer's projections into attention and the pools, in one launch: q and k
+ * rows (token t, head h at q + t * q_stride_token + h * q_stride_head, in
+ * elements; rows contiguous) are RMS-normalised over head_dim with weight
+ * q_weight / k_weight [head_dim] (NULL: not) and eps, their first rotary_dim
+ * elements turned by the angle positions[t] * inv_freq[i] of pair i and scaled
+ * by attention_factor; pair i is elements (i, i + rotary_dim / 2), or
+ * (2i, 2i + 1) when interleaved.  q rows go to q_out [num_tokens, num_q_heads,
+ * head_dim] (may be q itself when q is contiguous), k and v rows to the pools
+ * at position targets[t].  Arithmetic in f32 with one rounding; angles in f64.
+ * targets[t] = -1 stores nothing for token t (padding); targets outside
+ * [-1, pool_tokens) are skipped and TA_ERR_BOUNDS is OR-ed into *status.  The
+ * targets >= 0 have to be distinct.  klen .. num_jobs: the tails' lengths, as
+ * in ta_decode_append.  head_dim 32, 64 or 128; rotary_dim a multiple of 16 up
+ * to head_dim; rows 16-byte aligned (strides multiples of 8 elements).
+ */
+int ta_rotary_append(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k,
+                     int64_t k_stride_token, int64_t k_stride_head, const void* v, int64_t v_stride_token,
+                     int64_t v_stride_head, const int64_t* positions, const float* inv_freq, int32_t rotary_dim,
+                     int32_t interleaved, float attention_factor, const void* q_weight, const void* k_weight,
+                     float eps, void* q_out, void* kpool, void* vpool, const int64_t* targets, int32_t num_tokens,
+                     int32_t num_q_heads, int32_t num_kv_heads, int64_t pool_tokens, int32_t head_dim, int32_t dtype,
+                     int32_t* klen, const int32_t* tail_jobs, int32_t num_tails, const int64_t* count, int32_t offset,
+                     int32_t num_jobs, int32_t* status, void* stream);
+
+/*
+ * Attention of a ragged batch of chunks of new tokens over their sequences'
+ * pages of the pools.  Sequence b has the query rows [cu_q[b], cu_q[b+1]) of q
+ * (cu_q [num_seqs + 1] on the device, rising) and kv_lens[b] keys, its new
+ * tokens' own among them; key j lies at pool position table[b * table_stride +
+ * j / page_size] * page_size + j % page_size (page_size a power of two).  Row i
+ * of n attends the first kv_lens[b] - n + i + 1 keys when causal, else all.
+ * out [num_tokens, num_q_heads, head_dim] (dtype of q) and, when not NULL,
+ * out_lse [num_tokens, num_q_heads] (natural log) are written for the rows of
+ * the sequences alone: rows outside [cu_q[0], cu_q[num_seqs]) stay as they are.
+ * A row without keys gets out = 0 and LSE = -inf.  K and V of keys below
+ * kv_lens have to be finite; pool positions past them may hold anything.
+ * Query rows as in ta_rotary_append; scale > 0.  workspace: at least
+ * ta_chunk_workspace_bytes (16-byte aligned; 0 bytes: may be NULL), used by
+ * this call alone until it has run.  TA_ERR_BOUNDS in *status: a length beyond
+ * the table (clamped), a sequence outside q (skipped), a position outside the
+ * pools (its key read as zeros).
+ */
+int64_t ta_chunk_workspace_bytes(int32_t num_tokens, int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
+                                 int32_t head_dim, int32_t table_width, int32_t page_size);
+int ta_chunk_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* kpool,
+                       const void* vpool, int64_t pool_tokens, const int32_t* table, int64_t table_stride,
+                       int32_t table_width, int32_t page_size, const int32_t* kv_lens, const int32_t* cu_q,
+                       int32_t num_seqs, int32_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                       int32_t head_dim, int32_t dtype, float scale, int32_t causal, void* out, float* out_lse,
+                       void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+
+/*
+ * Beam search's selection.  logits: num_requests * num_beams rows of vocab
+ * values (bf16, f16 or f32; row_stride elements apart), scores [num_requests,
+ * num_beams] f32.  A candidate (beam w, token t) scores scores[w] + logits[w, t]
+ * - logsumexp(logits[w, :]); each request's k best go to out_scores (f32),
+ * out_parents and out_tokens [num_requests, k], best first, ties to the lowest
+ * w * vocab + t (scores are compared in f64).  A beam with finished[w] != 0
+ * (finished may be NULL) offers end_token alone, at its unchanged score, its
+ * other candidates at -inf.  A logit NaN counts as -inf, +inf as the largest
+ * f32; a beam score NaN as -inf.  k and num_beams at most 32, k at most
+ * num_beams * vocab.  workspace: ta_beam_workspace_bytes, 16-byte aligned, used
+ * by this call alone until it has run.
+ */
+int64_t ta_beam_workspace_bytes(int32_t num_requests, int32_t num_beams, int32_t vocab, int32_t k, int32_t dtype);
+int ta_beam_select(const void* logits, int64_t row_stride, const float* scores, const uint8_t* finished,
+                   int32_t num_requests, int32_t num_beams, int32_t vocab, int32_t k, int32_t end_token, int32_t dtype,
+                   float* out_scores, int64_t* out_parents, int64_t* out_tokens, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/*
+ * The beams' states after a selection: out[r, i, :] = states[r, parents[r, i], :]
+ * for rows of row_bytes bytes.  Strides of states in bytes, of parents in
+ * elements; out [num_requests, kept, row_bytes] contiguous, not overlapping
+ * states.  A parent outside [0, num_beams) leaves its row as it is and ORs
+ * TA_ERR_BOUNDS into *status.
+ */
+int ta_beam_reorder(const void* states, int64_t stride_request, int64_t stride_beam, int32_t num_requests,
+                    int32_t num_beams, int64_t row_bytes, const int64_t* parents, int64_t parent_stride, int32_t kept,
+                    void* out, int32_t* status, void* stream);
 
 /*
  * Host-side plan builder: the metadata buffer and layout of a physical job list

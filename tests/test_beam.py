@@ -1,0 +1,253 @@
+"""Beam selection and the reordering of states (``tree_attention.beam``).
+
+Parents and tokens must equal those of a 64-bit sort (ties to the lowest beam *
+vocabulary + token) wherever the neighbouring exact scores lie further apart than
+the kernel's own error; scores are within ``2^-24 |score| + 2^-20``: one rounding
+to f32, and a log of a sum whose f32 terms are within 2^-21 each.
+"""
+import math
+
+import pytest
+import torch
+
+from tree_attention import _lib
+
+DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+ERR = 2.0 ** -20
+
+
+def reference(logits, scores, finished=None, end=-1):
+    """(scores, w * V + t) of every request's candidates, sorted, in 64 bits on the CPU."""
+    x = logits.cpu().double().nan_to_num(nan=-math.inf, posinf=torch.finfo(torch.float32).max, neginf=-math.inf)
+    s = scores.cpu().double().nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf)
+    r, w, v = x.shape
+    top = x.amax(-1, keepdim=True)
+    shifted = torch.where(top > -math.inf, x - top, -math.inf)
+    lse = shifted.exp().sum(-1, keepdim=True).log()
+    cand = torch.where(shifted > -math.inf, shifted - lse, -math.inf) + s[..., None]
+    if finished is not None:
+        ended = torch.where(torch.arange(v) == end, s[..., None], -math.inf)
+        cand = torch.where(finished.cpu()[..., None], ended, cand)
+    return cand.reshape(r, w * v).sort(dim=1, descending=True, stable=True)
+
+
+def check(logits, scores, k, finished=None, end=-1):
+    from tree_attention.beam import beam_select
+    got, parents, tokens = (t.cpu() for t in beam_select(logits, scores, k, finished=finished, end_token=end))
+    torch.cuda.synchronize()
+    want, order = reference(logits if logits.dim() == 3 else logits.view(*scores.shape, -1), scores, finished, end)
+    exact = want[:, :k]
+    finite = exact > -math.inf
+    assert torch.equal(got > -math.inf, finite)
+    assert torch.all((got.double() - exact)[finite].abs() <= 2.0 ** -24 * exact[finite].abs() + ERR)
+    # Candidates whose exact scores lie within the error of one another form a run.  Unequal beams' sums
+    # are rounded apart (a relative 2^-53 already in 64 bits), so their order within a run is open, down to
+    # candidates that are equal in real numbers; within one beam, and between beams of equal rows and scores, it is not.
+    rows = logits.reshape(*scores.shape, -1).cpu()
+    vocab = rows.shape[-1]
+    for r in range(len(scores)):
+        twin = [min(j for j in range(w + 1) if j == w or (
+            scores[r, j] == scores[r, w] and torch.equal(rows[r, j], rows[r, w])
+            and (finished is None or finished[r, j] == finished[r, w]))) for w in range(scores.shape[1])]
+        mine = (parents[r] * vocab + tokens[r]).tolist()
+        assert len(set(mine)) == k
+        ends = (~(want[r, :-1] - want[r, 1:] < 4 * ERR) & (want[r, :-1] > -math.inf)).nonzero().flatten() + 1
+        ends = ends.tolist() + [want.shape[1]]
+        first = 0
+        for i in ends:
+            run, got_run = order[r, first:i].tolist(), mine[first:i]
+            if i <= k:
+                assert sorted(run) == sorted(got_run)
+            if len({twin[f // vocab] for f in run}) == 1 or not want[r, first] > -math.inf:
+                assert run[:len(got_run)] == got_run          # cut by k: the lowest come first
+            else:
+                assert set(got_run) <= set(run)
+            first = i
+            if first >= k:
+                break
+
+
+# ---- on the CPU ------------------------------------------------------------------
+def test_validation_without_gpu():
+    lib = _lib.load()
+    p = 4096
+
+    def select(logits=p, stride=1000, scores=p, finished=None, r=2, w=4, v=1000, k=8, end=-1, dtype=_lib.DTYPE_F32, out=p,
+               ws=p, size=1 << 40):
+        return lib.ta_beam_select(logits, stride, scores, finished, r, w, v, k, end, dtype, out, p, p, ws, size, None)
+
+    for bad in (dict(dtype=9), dict(w=33), dict(k=33), dict(v=(1 << 30) + 1)):
+        assert select(**bad) == _lib.ERR_UNSUPPORTED, bad
+    for bad in (dict(r=-1), dict(w=0), dict(v=0), dict(k=0), dict(stride=-1), dict(w=1, v=4), dict(finished=p),
+                dict(finished=p, end=1000), dict(logits=None), dict(logits=p + 2), dict(scores=None), dict(out=None),
+                dict(ws=None), dict(ws=p + 8)):
+        assert select(**bad) == _lib.ERR_ARG, bad
+    need = lib.ta_beam_workspace_bytes(2, 4, 1000, 8, _lib.DTYPE_F32)
+    assert need > 0 and select(size=need - 1) == _lib.ERR_TOO_LARGE
+    assert select(r=0) == 0                                  # nothing to do, nothing launched
+
+    def reorder(states=p, sr=64, sb=16, r=2, w=4, size=16, parents=p, ps=4, kept=4, out=p):
+        return lib.ta_beam_reorder(states, sr, sb, r, w, size, parents, ps, kept, out, None, None)
+
+    for bad in (dict(states=None), dict(parents=None), dict(out=None), dict(r=-1), dict(w=0), dict(kept=-1),
+                dict(size=-1), dict(sr=-1), dict(sb=-1), dict(ps=-1)):
+        assert reorder(**bad) == _lib.ERR_ARG, bad
+    assert reorder(kept=1 << 17) == _lib.ERR_UNSUPPORTED
+    assert reorder(r=0) == reorder(kept=0) == reorder(size=0) == 0
+
+
+# ---- on the GPU ------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("r,w,v,k", [(1, 1, 1, 1), (1, 1, 7, 7), (2, 3, 31, 5), (3, 4, 1000, 8), (5, 2, 8191, 4),
+                                     (2, 4, 8193, 32), (1, 32, 20011, 32), (17, 5, 50257, 10), (2, 8, 152000, 16)])
+def test_select(r, w, v, k, dtype):
+    g = torch.Generator().manual_seed(r * 100 + w)
+    logits = (torch.randn(r, w, v, generator=g) * 3).to(DTYPES[dtype]).cuda()
+    scores = (-20 * torch.rand(r, w, generator=g)).cuda()
+    check(logits, scores, k)
+    check(logits.view(r * w, v), scores, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_ties_go_to_the_lowest_index(dtype):
+    """All logits equal; few distinct values; equal beams; a run of equal maxima across slices."""
+    for v in (5, 300, 20000):
+        same = torch.full((2, 3, v), 1.5, dtype=DTYPES[dtype], device="cuda")
+        scores = torch.tensor([[0.0, 0.0, 0.0], [-2.0, -1.0, -1.0]], device="cuda")
+        check(same, scores, 4)
+        few = torch.randint(0, 3, (2, 3, v), generator=torch.Generator().manual_seed(v)).to(DTYPES[dtype]).cuda()
+        check(few[:, :1].expand(-1, 3, -1).contiguous(), scores, 12)
+        check(few, scores, 12)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["rising", "falling", "one warp"])
+def test_sorted_logits(order):
+    """Orders that defeat a bound taken from thread maxima."""
+    v = 30000
+    x = torch.linspace(-9, 9, v)
+    if order == "falling":
+        x = x.flip(0)
+    if order == "one warp":
+        x = torch.where(torch.arange(v) // 8 % 256 < 32, 5 + x / 100, -50 + x)
+    logits = x.repeat(2, 3, 1).cuda()
+    check(logits, torch.tensor([[0.0, -0.5, -1.0], [-3.0, -1.1, -7.0]], device="cuda"), 32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_masks_dead_and_finished_beams(dtype):
+    r, w, v = 4, 5, 9000
+    g = torch.Generator().manual_seed(7)
+    logits = (torch.randn(r, w, v, generator=g) * 2).to(DTYPES[dtype])
+    logits[:, :, torch.rand(v, generator=g) < 0.9] = -math.inf
+    logits[1, 2] = -math.inf                                 # nothing is allowed
+    logits[2] = -math.inf
+    logits[2, 1, 8191] = logits[2, 1, 17] = 3.0              # two candidates in all
+    scores = -5 * torch.rand(r, w, generator=g)
+    scores[0, 1:] = -math.inf                                # a first step: one live beam
+    scores[3, 4] = float("nan")
+    finished = torch.zeros(r, w, dtype=torch.bool)
+    logits, scores = logits.cuda(), scores.cuda()
+    check(logits, scores, 10)
+    finished[0, 0] = finished[1, 3] = finished[3, 4] = True
+    finished[2] = True
+    for end in (0, 17, v - 1):
+        check(logits, scores, 10, finished.cuda(), end)
+
+
+@pytest.mark.gpu
+def test_nan_and_infinite_logits():
+    g = torch.Generator().manual_seed(8)
+    logits = torch.randn(3, 4, 10000, generator=g)
+    logits[0, 1, 100:200] = float("nan")
+    logits[1, 2, 9000] = math.inf
+    logits[1, 3, [5, 9999]] = math.inf
+    logits[2, 0] = float("nan")
+    check(logits.cuda(), -3 * torch.rand(3, 4, generator=g).cuda(), 6)
+
+
+@pytest.mark.gpu
+def test_strided_and_unaligned_rows():
+    g = torch.Generator().manual_seed(9)
+    whole = torch.randn(3, 4, 5003, generator=g).bfloat16().cuda()
+    scores = -3 * torch.rand(3, 4, generator=g).cuda()
+    check(whole[..., 1:], scores, 8)
+    check(whole[..., 3:4098], scores, 8)
+    check(whole[:, 1:3], scores[:, 1:3], 8)
+    check(whole[:, :1], scores[:, :1], 8)
+    check(whole.transpose(0, 1), scores.T, 8)
+    check(whole.transpose(1, 2).contiguous().transpose(1, 2), scores, 8)
+    check(whole[:, :1].expand(-1, 4, -1), scores, 8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,length", [(torch.int32, 1), (torch.int32, 257), (torch.int64, 4096), (torch.bfloat16, 3),
+                                          (torch.uint8, 5), (torch.float32, 100000)])
+def test_reorder(dtype, length):
+    from tree_attention.beam import beam_reorder
+    g = torch.Generator().manual_seed(length)
+    states = torch.randint(0, 100, (3, 5, length), generator=g).to(dtype).cuda()
+    parents = torch.randint(0, 5, (3, 8), generator=g).cuda()
+    want = states.gather(1, parents[..., None].expand(-1, -1, length))
+    assert torch.equal(beam_reorder(states, parents), want)
+    assert torch.equal(beam_reorder(states, parents[:, 2:5]), want[:, 2:5])
+    assert torch.equal(beam_reorder(states.transpose(0, 1).contiguous().transpose(0, 1), parents), want)
+    assert torch.equal(beam_reorder(states[..., None], parents)[..., 0], want)
+    out = torch.empty_like(want)
+    assert beam_reorder(states, parents, out=out) is out and torch.equal(out, want)
+
+
+@pytest.mark.gpu
+def test_reorder_records_bad_parents():
+    from tree_attention.beam import beam_reorder
+    states = torch.arange(24, device="cuda").view(2, 3, 4)
+    out = torch.full((2, 3, 4), -1, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    beam_reorder(states, torch.tensor([[0, 3, 1], [2, -1, 2]]).cuda(), out=out, status=status)
+    assert int(status) == _lib.ERR_BOUNDS
+    assert torch.equal(out[0, 1], torch.full((4,), -1).cuda()) and torch.equal(out[1, 1], out[0, 1])
+    assert torch.equal(out[0, [0, 2]], states[0, [0, 1]]) and torch.equal(out[1, [0, 2]], states[1, [2, 2]])
+
+
+@pytest.mark.gpu
+def test_captured_selection_follows_its_inputs():
+    from tree_attention.beam import beam_reorder, beam_select
+    g = torch.Generator().manual_seed(10)
+    logits, scores = torch.randn(4, 3, 12000, generator=g).cuda(), -torch.rand(4, 3, generator=g).cuda()
+    states = torch.arange(4 * 3 * 8, device="cuda", dtype=torch.int32).view(4, 3, 8)
+    beam_select(logits, scores)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = beam_select(logits, scores)
+        moved = beam_reorder(states, got[1])
+    for seed in (1, 2):
+        logits.copy_(torch.randn(4, 3, 12000, generator=g.manual_seed(seed)))
+        graph.replay()
+        eager = beam_select(logits, scores)
+        assert all(torch.equal(a, b) for a, b in zip(got, eager))
+        assert torch.equal(moved, beam_reorder(states, eager[1]))
+
+
+@pytest.mark.gpu
+def test_refusals_on_gpu():
+    from tree_attention.beam import beam_reorder, beam_select
+    logits, scores = torch.zeros(2, 3, 10, device="cuda"), torch.zeros(2, 3, device="cuda")
+    done = torch.zeros(2, 3, dtype=torch.bool, device="cuda")
+    for args in ((logits.cpu(), scores.cpu()), (logits, scores.cpu()), (logits, scores.double()), (logits[:1], scores),
+                 (logits.long(), scores), (logits, scores, 0), (logits, scores, 33), (logits[..., :1], scores, 4),
+                 (torch.zeros(2, 33, 4).cuda(), torch.zeros(2, 33).cuda())):
+        with pytest.raises(ValueError):
+            beam_select(*args)
+    for kwargs in (dict(finished=done), dict(finished=done, end_token=10), dict(finished=done.int(), end_token=1),
+                   dict(finished=done[:1], end_token=1)):
+        with pytest.raises(ValueError):
+            beam_select(logits, scores, **kwargs)
+    assert beam_select(logits[:0], scores[:0])[0].shape == (0, 3)
+    states, parents = torch.zeros(2, 3, 4, device="cuda"), torch.zeros(2, 3, dtype=torch.int64, device="cuda")
+    for args in ((states, parents.int()), (states, parents[:1]), (states, parents.cpu()), (states[0], parents),
+                 (states, parents, states), (states, parents, torch.empty(2, 3, 5).cuda())):
+        with pytest.raises(ValueError):
+            beam_reorder(*args)

@@ -1,0 +1,317 @@
+"""Attention of chunks of new tokens over pages of the pools (``tree_attention.chunk``).
+
+Checked against the definition in 64 bits.  Tolerances: each softmax weight is
+rounded once to the input type (relative ``eps / 2``) before the value product
+and the output once more, so an output is off by at most
+``eps / 2 * (sum_j w_j |v_j| + |out|)``; the f32 parts (a dot product of D terms,
+ex2 and lg2 at 2^-22, f32 sums) add ``2^-24 (D + 8) sum |q k| scale`` to a score and
+``2^-20`` relative to a sum, which the terms below carry for outputs and LSEs.
+"""
+import math
+
+import pytest
+import torch
+
+from tree_attention import _lib
+
+DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def make_batch(fresh, total, hq, hk, dim, page, dtype, seed, device="cuda", slack=3, garbage=True):
+    """Random queries and pools; pages in random order; unused positions hold NaN."""
+    g = torch.Generator().manual_seed(seed)
+    pages = [-(-t // page) for t in total]
+    pool = sum(pages) + slack
+    order = torch.randperm(pool, generator=g)
+    table = torch.full((len(fresh), max(1, max(pages, default=1))), -1, dtype=torch.int32)
+    kp = torch.randn(hk, pool * page, dim, generator=g).to(dtype)
+    vp = torch.randn(hk, pool * page, dim, generator=g).to(dtype)
+    used = torch.zeros(pool * page, dtype=torch.bool)
+    at, paths = 0, []
+    for b, (count, t) in enumerate(zip(pages, total)):
+        own = order[at:at + count]
+        at += count
+        table[b, :count] = own.int()
+        path = (own[:, None] * page + torch.arange(page)).flatten()[:t]
+        used[path] = True
+        paths.append(path)
+    if garbage:
+        kp[:, ~used] = float("nan")
+        vp[:, ~used] = float("nan")
+    q = (torch.randn(sum(fresh), hq, dim, generator=g) * 2).to(dtype)
+    cu = torch.tensor([0] + list(fresh)).cumsum(0).int()
+    lens = torch.tensor(total, dtype=torch.int32)
+    return dict(q=q.to(device), kp=kp.to(device), vp=vp.to(device), table=table.to(device), lens=lens.to(device),
+                cu=cu.to(device), paths=paths, page=page)
+
+
+def reference(batch, causal=True, scale=None):
+    """(out, lse, output tolerance without the type's part, LSE tolerance, sum_j w_j |v_j|) in 64 bits on the CPU."""
+    q, kp, vp = batch["q"].cpu().double(), batch["kp"].cpu().double(), batch["vp"].cpu().double()
+    cu = batch["cu"].tolist()
+    n, hq, dim = q.shape
+    group = hq // kp.shape[0]
+    scale = dim ** -0.5 if scale is None else scale
+    out, mass = torch.zeros_like(q), torch.zeros_like(q)
+    lse = torch.full((n, hq), -math.inf, dtype=torch.float64)
+    err = torch.zeros((n, hq), dtype=torch.float64)
+    for b, path in enumerate(batch["paths"]):
+        rows, keys = slice(cu[b], cu[b + 1]), len(path)
+        count = cu[b + 1] - cu[b]
+        if not count or not keys:
+            continue
+        k, v = kp[:, path].repeat_interleave(group, 0), vp[:, path].repeat_interleave(group, 0)
+        limit = keys - count + 1 + torch.arange(count) if causal else torch.full((count,), keys)
+        hidden = torch.arange(keys) >= limit[:, None]
+        s = (torch.einsum("nhd,hkd->hnk", q[rows], k) * scale).masked_fill(hidden, -math.inf)
+        lse[rows] = torch.logsumexp(s, -1).T
+        w = torch.softmax(s, -1).nan_to_num(nan=0.0)
+        out[rows] = torch.einsum("hnk,hkd->nhd", w, v)
+        mass[rows] = torch.einsum("hnk,hkd->nhd", w, v.abs())
+        reach = torch.einsum("nhd,hkd->hnk", q[rows].abs(), k.abs()).masked_fill(hidden, 0.0).amax(-1) * scale
+        err[rows] = 2.0 ** -24 * (dim + 8) * reach.T
+    return out, lse, err, 2 * err + 2.0 ** -20 * (1 + lse.abs().nan_to_num(posinf=0.0)), mass
+
+
+def check(batch, out, lse, causal=True, scale=None):
+    want, want_lse, err, lse_tol, mass = reference(batch, causal, scale)
+    half = torch.finfo(out.dtype).eps / 2
+    tiny = torch.finfo(out.dtype).smallest_normal * torch.finfo(out.dtype).eps
+    tol = half * (mass + want.abs() + half * mass) + (2 * err[..., None] + 2.0 ** -20) * mass + tiny
+    off = (out.cpu().double() - want).abs()
+    assert torch.all(off <= tol), f"worst {(off / tol.clamp(min=1e-30)).max():.3f} of the tolerance"
+    got = lse.cpu().double()
+    assert torch.equal(got == -math.inf, want_lse == -math.inf)
+    seen = want_lse > -math.inf
+    assert torch.all((got - want_lse)[seen].abs() <= lse_tol[seen])
+
+
+def run(batch, **kwargs):
+    from tree_attention.chunk import chunk_attention
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    lse = torch.full(batch["q"].shape[:2], 7.0, device="cuda")
+    out = chunk_attention(batch["q"], batch["kp"], batch["vp"], batch["table"], batch["lens"], batch["cu"],
+                          page_size=batch["page"], out_lse=lse, status=status, **kwargs)
+    torch.cuda.synchronize()
+    assert int(status) == 0
+    return out, lse
+
+
+# ---- on the CPU: refusals ------------------------------------------------------
+def test_validation_without_gpu():
+    lib = _lib.load()
+    p = 4096
+
+    def call(q=p, st=4096, sh=128, kp=p, tokens=64, table=p, width=8, page=16, lens=p, cu=p, b=2, n=4, hq=32, hk=8,
+             dim=128, dtype=_lib.DTYPE_BF16, scale=0.1, out=p, ws=p, ws_bytes=1 << 40):
+        return lib.ta_chunk_attention(q, st, sh, kp, p, tokens, table, width, width, page, lens, cu, b, n, hq, hk, dim,
+                                      dtype, scale, 1, out, None, ws, ws_bytes, None, None)
+
+    for bad in (dict(dtype=3), dict(dim=96), dict(width=1 << 30, page=1024), dict(tokens=1 << 32)):
+        assert call(**bad) == _lib.ERR_UNSUPPORTED, bad
+    for bad in (dict(page=3), dict(page=0), dict(hq=30), dict(hk=0), dict(n=-1), dict(b=-1), dict(scale=0.0),
+                dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan), dict(q=None), dict(kp=None),
+                dict(table=None), dict(lens=None), dict(cu=None), dict(out=None), dict(q=4104), dict(out=4100),
+                dict(kp=4104), dict(sh=132), dict(st=-8), dict(tokens=-1)):
+        assert call(**bad) == _lib.ERR_ARG, bad
+    assert call(n=0) == 0 and call(b=0) == 0                 # nothing to do, nothing launched
+    # one token over a long table is split: without its workspace the call is refused
+    need = lib.ta_chunk_workspace_bytes(1, 1, 32, 8, 128, 8192, 1)
+    assert need > 0 and need % (32 * 129 * 4) == 0
+    assert call(n=1, b=1, width=8192, page=1, ws_bytes=need - 1) == _lib.ERR_TOO_LARGE
+    assert call(n=1, b=1, width=8192, page=1, ws=None) == _lib.ERR_ARG
+
+
+def test_python_refusals():
+    from tree_attention.chunk import chunk_attention, path_table
+    with pytest.raises(ValueError):                          # CPU tensors
+        chunk_attention(torch.zeros(1, 2, 64).bfloat16(), *[torch.zeros(1, 4, 64).bfloat16()] * 2,
+                        torch.zeros(1, 4).int(), torch.ones(1).int(), torch.tensor([0, 1]).int())
+    table, lens = path_table([[3, 4, 9], [1], []], "cpu")
+    assert table.tolist() == [[3, 4, 9], [1, -1, -1], [-1, -1, -1]] and lens.tolist() == [3, 1, 0]
+    table, lens = path_table([], "cpu")
+    assert table.shape == (0, 1) and lens.shape == (0,)
+
+
+# ---- on the GPU ------------------------------------------------------------------
+SHAPES = [(32, 8, 128), (8, 8, 128), (24, 8, 64), (12, 2, 64), (4, 2, 32), (16, 1, 128), (7, 1, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_one_token(shape, dtype):
+    """Contexts of one key, around a tile's end and of several tiles and splits."""
+    for i, keys in enumerate((1, 2, 127, 128, 129, 256, 257, 700)):
+        batch = make_batch([1], [keys], *shape, 1, DTYPES[dtype], 10 + i)
+        check(batch, *run(batch))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [1, 2, 16, 64, 256])
+@pytest.mark.parametrize("shape", [(32, 8, 128), (12, 2, 64)], ids=["d128", "d64"])
+def test_ragged_batch(shape, page):
+    """Chunks and contexts of unlike lengths, pages that end inside a tile, empty sequences."""
+    fresh = [1, 0, 37, 128, 5, 65, 1, 3, 130]
+    total = [300, 0, 37, 200, 1000, 65, 1, 129, 259]
+    batch = make_batch(fresh, total, *shape, page, torch.bfloat16, 3)
+    check(batch, *run(batch))
+    out, lse = run(batch, causal=False)
+    check(batch, out, lse, causal=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("fresh,total", [(64, 64), (65, 65), (257, 600), (300, 1500)])
+@pytest.mark.parametrize("shape", [(32, 8, 128), (4, 4, 128), (6, 2, 64), (4, 2, 32)], ids=lambda s: "x".join(map(str, s)))
+def test_chunk(shape, fresh, total, dtype):
+    batch = make_batch([fresh], [total], *shape, 1, DTYPES[dtype], fresh)
+    check(batch, *run(batch))
+
+
+@pytest.mark.gpu
+def test_rows_without_keys():
+    """A chunk longer than its keys: the first rows see nothing; a sequence without keys at all."""
+    batch = make_batch([200, 4, 1], [150, 0, 1], 8, 2, 128, 16, torch.bfloat16, 5)
+    out, lse = run(batch)
+    assert torch.equal(out[:50], torch.zeros_like(out[:50])) and torch.all(lse[:50] == -math.inf)
+    assert torch.equal(out[200:204], torch.zeros_like(out[200:204])) and torch.all(lse[200:204] == -math.inf)
+    check(batch, out, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("keys", [100, 1200])
+def test_large_scores(keys):
+    """Scores that rise along the keys (each tile raises the maximum) and a given scale."""
+    batch = make_batch([3, 200], [keys, keys], 8, 2, 128, 1, torch.bfloat16, 6)
+    ramp = torch.zeros_like(batch["kp"])
+    for path in batch["paths"]:
+        ramp[:, path, 0] = torch.linspace(-40, 40, keys, device="cuda").to(ramp.dtype)
+    batch["kp"] = (batch["kp"].nan_to_num() + ramp)
+    batch["q"][..., 0] = 4
+    check(batch, *run(batch))
+    out, lse = run(batch, scale=0.3)
+    check(batch, out, lse, scale=0.3)
+
+
+@pytest.mark.gpu
+def test_rows_behind_the_last_sequence_and_strides():
+    """Padding rows of out and out_lse stay; queries may be a strided slice; tables wider than needed."""
+    from tree_attention.chunk import chunk_attention
+    batch = make_batch([5, 70], [40, 300], 8, 2, 64, 1, torch.float16, 8)
+    n = batch["q"].shape[0]
+    wide = torch.randn(n + 9, 12, 64, device="cuda").half()
+    wide[:n, 2:10] = batch["q"]
+    out = torch.full((n + 9, 8, 64), 3.0, device="cuda", dtype=torch.float16)
+    lse = torch.full((n + 9, 8), 5.0, device="cuda")
+    table = torch.full((2, 1000), -1, dtype=torch.int32, device="cuda")
+    table[:, :batch["table"].shape[1]] = batch["table"]
+    got = chunk_attention(wide[:, 2:10], batch["kp"], batch["vp"], table, batch["lens"], batch["cu"], out=out,
+                          out_lse=lse)
+    assert got is out
+    assert torch.all(out[n:] == 3) and torch.all(lse[n:] == 5)
+    check(batch, out[:n], lse[:n])
+    # misaligned rows are copied first
+    odd = torch.randn(n, 8, 65, device="cuda").half()
+    odd[..., 1:] = batch["q"]
+    lse = torch.empty((n, 8), device="cuda")
+    check(batch, chunk_attention(odd[..., 1:], batch["kp"], batch["vp"], batch["table"], batch["lens"], batch["cu"],
+                                 out_lse=lse), lse)
+
+
+@pytest.mark.gpu
+def test_bad_pages_and_lengths_are_recorded():
+    from tree_attention.chunk import chunk_attention
+    batch = make_batch([4, 6], [64, 200], 8, 2, 64, 16, torch.bfloat16, 9, garbage=False)
+    good, _ = run(batch)
+    args = [batch["q"], batch["kp"], batch["vp"], batch["table"], batch["lens"], batch["cu"]]
+
+    def call(index, value):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        out = chunk_attention(*[value if i == index else a for i, a in enumerate(args)], page_size=16, status=status)
+        torch.cuda.synchronize()
+        return out, int(status)
+
+    for entry in (-1, 10 ** 6, -2 ** 31):
+        table = batch["table"].clone()
+        table[1, 2] = entry
+        out, code = call(3, table)
+        assert code == _lib.ERR_BOUNDS and torch.equal(out[:4], good[:4])   # the other sequence is as it was
+    out, code = call(4, torch.tensor([64, 10 ** 6], dtype=torch.int32, device="cuda"))
+    assert code == _lib.ERR_BOUNDS and torch.equal(out[:4], good[:4])
+    out, code = call(4, torch.tensor([64, -5], dtype=torch.int32, device="cuda"))
+    assert code == _lib.ERR_BOUNDS and torch.equal(out[:4], good[:4]) and not out[4:].any()
+    _, code = call(5, torch.tensor([0, 4, 11], dtype=torch.int32, device="cuda"))
+    assert code == _lib.ERR_BOUNDS
+
+
+@pytest.mark.gpu
+def test_captured_call_follows_its_tensors_and_streams():
+    """A graph replays with new lengths, tables and queries; two graphs and an eager call do not share scratch."""
+    from tree_attention.chunk import chunk_attention
+    a = make_batch([1] * 6, [900, 20, 333, 128, 1, 640], 8, 2, 128, 1, torch.bfloat16, 11)
+    b = make_batch([1] * 6, [17, 900, 200, 555, 128, 3], 8, 2, 128, 1, torch.bfloat16, 12, slack=63)
+    names = ("q", "kp", "vp", "table", "lens", "cu")
+    pools = max(a["kp"].shape[1], b["kp"].shape[1])
+
+    def grown(x):
+        return torch.nn.functional.pad(x, (0, 0, 0, pools - x.shape[1]))
+
+    live = {n: (grown(a[n]) if n in ("kp", "vp") else a[n]).clone() for n in names}
+    lse = torch.empty(6, 8, device="cuda")
+    chunk_attention(*[live[n] for n in names], out_lse=lse)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = chunk_attention(*[live[n] for n in names], out_lse=lse)
+        graphs.append((graph, out))
+    for batch in (b, a, b):
+        for n in names:
+            live[n].copy_(grown(batch[n]) if n in ("kp", "vp") else batch[n])
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for (graph, _), stream in zip(graphs, streams):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            check(batch, out, lse)
+
+
+@pytest.mark.gpu
+def test_far_positions_of_a_large_pool():
+    """Element offsets past 32 bits: positions near the end of a pool of 2^31 elements and more a head."""
+    from tree_attention.chunk import chunk_attention
+    tokens, dim = (1 << 25) + 1000, 64                       # 2^31 elements and a little in one head
+    kp = torch.zeros(1, tokens, dim, device="cuda", dtype=torch.bfloat16)
+    vp = torch.zeros_like(kp)
+    g = torch.Generator().manual_seed(13)
+    keys = 300
+    kp[0, -keys:] = torch.randn(keys, dim, generator=g).bfloat16().cuda()
+    vp[0, -keys:] = torch.randn(keys, dim, generator=g).bfloat16().cuda()
+    q = torch.randn(2, 4, dim, generator=g).bfloat16().cuda()
+    table = torch.arange(tokens - keys, tokens, device="cuda", dtype=torch.int32)[None]
+    lens, cu = torch.tensor([keys], device="cuda").int(), torch.tensor([0, 2], device="cuda").int()
+    lse = torch.empty(2, 4, device="cuda")
+    out = chunk_attention(q, kp, vp, table, lens, cu, out_lse=lse)
+    small = dict(q=q, kp=kp[:, -keys:], vp=vp[:, -keys:], cu=cu, paths=[torch.arange(keys)])
+    check(small, out, lse)
+
+
+@pytest.mark.gpu
+def test_refusals_on_gpu():
+    from tree_attention.chunk import chunk_attention
+    b = make_batch([2], [40], 8, 2, 64, 16, torch.bfloat16, 14)
+    good = dict(q=b["q"], kp=b["kp"], vp=b["vp"], table=b["table"], kv_lens=b["lens"], cu_q=b["cu"], page_size=16)
+    chunk_attention(**good)
+    for change in (dict(page_size=12), dict(page_size=0), dict(scale=0.0), dict(scale=-1.0), dict(q=b["q"].float()),
+                   dict(q=b["q"][:, :7]), dict(kp=b["kp"].half()), dict(kp=b["kp"][:, :-1]),
+                   dict(kp=b["kp"].transpose(0, 1), vp=b["vp"].transpose(0, 1)), dict(table=b["table"].long()),
+                   dict(table=b["table"][0]), dict(kv_lens=b["lens"].long()), dict(cu_q=b["cu"][:1]),
+                   dict(cu_q=b["cu"].cpu()), dict(out=b["q"]), dict(out=torch.empty_like(b["q"]).half()),
+                   dict(out_lse=torch.empty(2, 7, device="cuda")), dict(status=torch.zeros(1, device="cuda")),
+                   dict(q=b["q"][..., :48], kp=b["kp"][..., :48].contiguous(), vp=b["vp"][..., :48].contiguous())):
+        with pytest.raises(ValueError):
+            chunk_attention(**{**good, **change})
+    assert chunk_attention(**{**good, "q": b["q"][:0], "cu_q": torch.zeros(2, device="cuda").int()}).shape == (0, 8, 64)

@@ -91,28 +91,6 @@ __host__ __device__ constexpr uint32_t instr_desc(uint32_t ab_format, uint32_t b
   return umma_idesc(ab_format, 0, b_mn_major, kRows, kKeys);
 }
 
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));   // sm_100 three-input max
-  return d;
-}
-
-// Maximum of 128 values as a three-way tree: 65 max instructions, depth 5.
-__device__ __forceinline__ float max128(const float (&s)[kKeys]) {
-  float m[43];
-#pragma unroll
-  for (int i = 0; i < 42; ++i) m[i] = fmax3(s[3 * i], s[3 * i + 1], s[3 * i + 2]);
-  m[42] = fmaxf(s[126], s[127]);
-  float n[15];
-#pragma unroll
-  for (int i = 0; i < 14; ++i) n[i] = fmax3(m[3 * i], m[3 * i + 1], m[3 * i + 2]);
-  n[14] = m[42];
-  float o[5];
-#pragma unroll
-  for (int i = 0; i < 5; ++i) o[i] = fmax3(n[3 * i], n[3 * i + 1], n[3 * i + 2]);
-  return fmaxf(fmax3(o[0], o[1], o[2]), fmaxf(o[3], o[4]));
-}
-
 // 2^x for a pair on the FMA pipe: x = n + f with n = round(x) via the
 // 1.5 * 2^23 shift and f in [-0.5, 0.5]; 2^f by a degree-3 polynomial whose
 // coefficients are a Remez (minimax relative error) fit computed for this

@@ -279,6 +279,29 @@ __device__ __forceinline__ F2 splat(float x) {
   return r;
 }
 
+// ---- maxima -------------------------------------------------------------------
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));   // sm_100 three-input max
+  return d;
+}
+
+// Maximum of 128 values as a three-way tree: 65 max instructions, depth 5.
+__device__ __forceinline__ float max128(const float (&s)[128]) {
+  float m[43];
+#pragma unroll
+  for (int i = 0; i < 42; ++i) m[i] = fmax3(s[3 * i], s[3 * i + 1], s[3 * i + 2]);
+  m[42] = fmaxf(s[126], s[127]);
+  float n[15];
+#pragma unroll
+  for (int i = 0; i < 14; ++i) n[i] = fmax3(m[3 * i], m[3 * i + 1], m[3 * i + 2]);
+  n[14] = m[42];
+  float o[5];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) o[i] = fmax3(n[3 * i], n[3 * i + 1], n[3 * i + 2]);
+  return fmaxf(fmax3(o[0], o[1], o[2]), fmaxf(o[3], o[4]));
+}
+
 // ---- host side: tensor maps through the driver entry point -------------------
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,

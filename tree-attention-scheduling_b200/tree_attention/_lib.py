@@ -11,10 +11,11 @@ import os
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("libtree_attn_b200.so")
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 DTYPE_BF16 = 1
 DTYPE_F16 = 2
+DTYPE_F32 = 3
 
 ERR_ARG = 1
 ERR_LAUNCH = 2
@@ -32,7 +33,9 @@ STATUS_NAMES = {ERR_ARG: "invalid argument", ERR_LAUNCH: "kernel launch failed",
 
 # Every symbol declared in include/tree_attn.h.
 EXPORTS = ("ta_abi_version", "ta_error_string", "ta_segment", "ta_merge", "ta_attention",
-           "ta_attention_noalloc", "ta_update_tail_klen", "ta_decode_append", "ta_plan_build", "ta_schedule_tree")
+           "ta_attention_noalloc", "ta_update_tail_klen", "ta_decode_append", "ta_plan_build", "ta_schedule_tree",
+           "ta_rotary_append", "ta_chunk_workspace_bytes", "ta_chunk_attention", "ta_beam_workspace_bytes",
+           "ta_beam_select", "ta_beam_reorder")
 
 SCHEDULE_GREEDY = 1
 SCHEDULE_CUBE = 2
@@ -100,6 +103,21 @@ def load():
     lib.ta_schedule_tree.restype = ctypes.c_int
     lib.ta_schedule_tree.argtypes = [P, P, P, P, P, I32, I32, ctypes.POINTER(CostModelC), I32, I32, I32, P,
                                      ctypes.POINTER(ctypes.c_double)]
+    F32 = ctypes.c_float
+    lib.ta_rotary_append.restype = ctypes.c_int
+    lib.ta_rotary_append.argtypes = [P, I64, I64, P, I64, I64, P, I64, I64, P, P, I32, I32, F32, P, P, F32, P, P, P, P,
+                                     I32, I32, I32, I64, I32, I32, P, P, I32, P, I32, I32, P, P]
+    lib.ta_chunk_workspace_bytes.restype = I64
+    lib.ta_chunk_workspace_bytes.argtypes = [I32] * 7
+    lib.ta_chunk_attention.restype = ctypes.c_int
+    lib.ta_chunk_attention.argtypes = [P, I64, I64, P, P, I64, P, I64, I32, I32, P, P, I32, I32, I32, I32, I32, I32,
+                                       F32, I32, P, P, P, I64, P, P]
+    lib.ta_beam_workspace_bytes.restype = I64
+    lib.ta_beam_workspace_bytes.argtypes = [I32] * 5
+    lib.ta_beam_select.restype = ctypes.c_int
+    lib.ta_beam_select.argtypes = [P, I64, P, P, I32, I32, I32, I32, I32, I32, P, P, P, P, I64, P]
+    lib.ta_beam_reorder.restype = ctypes.c_int
+    lib.ta_beam_reorder.argtypes = [P, I64, I64, I32, I32, I64, P, I64, I32, P, P, P]
     version = lib.ta_abi_version()
     if version != ABI_VERSION:
         raise RuntimeError(f"kernel library ABI {version}, expected {ABI_VERSION}; rebuild it")
