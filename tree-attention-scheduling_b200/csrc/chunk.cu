@@ -11,10 +11,11 @@
 // over a range of its keys.  Roles:
 //
 //   warps 0-1   load K tiles (128 keys), warps 2-3 V tiles: warp w the tiles of
-//               parity w & 1 into ring slot w & 1.  Rows are gathered by
-//               16-byte cp.async into the 128-byte-swizzled layout the MMAs read,
-//               so any page size, order and fragmentation costs the same; keys
-//               past kv_b are filled with zeros
+//               parity w & 1 into ring slot w & 1.  A whole tile of pages of 16
+//               and more comes by TMA in boxes of a page's rows, one of smaller
+//               pages in a single box where its positions follow one another (those
+//               of a tree node do); anything else is gathered by 16-byte cp.async
+//               into the same 128-byte-swizzled layout, keys past kv_b as zeros
 //   warp 4      issues every tcgen05.mma (converged, one elected lane)
 //   warps 8-15  softmax: warpgroup t serves stream t, one thread per query row
 //
@@ -33,10 +34,13 @@
 //
 // When the (tile, KV head) pairs do not fill the GPU the keys are cut into
 // splits whose normalised f32 partials chunk_merge_kernel combines by LSE.
+// Batches of few rows a sequence (decode steps) run on the kernel of
+// chunk_rows.cu instead, with the same splits and merge.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
 
+#include "chunk_common.cuh"
 #include "ta_kernels.cuh"
 #include "tc_common.cuh"
 
@@ -56,35 +60,25 @@ constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;   // + stream * 128
 constexpr float kRescaleThreshold = 8.f;   // log2 units
 constexpr int kMaxSplits = 64;
 
-struct ChunkParams {
-  const uint16_t* q;
-  int64_t q_st, q_sh;                      // element strides: token, head
-  const uint16_t *k, *v;                   // [HK, T, D]
-  int64_t pool_tokens;
-  const int32_t* table;                    // [B, width]
-  int64_t table_stride;
-  const int32_t *lens, *cu;                // [B], [B + 1]
-  uint16_t* out;                           // [N, HQ, D]
-  float* lse;                              // [N, HQ] or null
-  float *part, *part_lse;                  // [splits, N, HQ, D], [splits, N, HQ] when splits > 1
-  int32_t* status;
-  float scale_log2;
-  int32_t width, page_shift, num_seqs, num_tokens, hq, group, causal, splits, split_tiles;
+// The pools [HK, T, D] as tensor maps, boxes of 64 columns x box_rows tokens.
+struct ChunkMaps {
+  CUtensorMap k, v;
 };
 
 template <int D>
 struct Smem {
   static constexpr uint32_t kTile = kRows * D * 2;
-  static constexpr uint32_t kBlock = D >= 64 ? kRows * 128 : kTile * 2;    // one 64-column swizzled block
-  static constexpr uint32_t kSlot = D >= 64 ? kTile : kRows * 128;         // D = 32 keeps 128-byte rows
+  static constexpr uint32_t kBlock = kRows * 128;                          // one 64-column swizzled block
+  static constexpr uint32_t kSlot = D >= 64 ? kTile : kBlock;              // D = 32 keeps 128-byte rows
   static constexpr uint32_t off_q = 0;
   static constexpr uint32_t off_k = off_q + 2 * kSlot;
   static constexpr uint32_t off_v = off_k + kStages * kSlot;
   static constexpr uint32_t off_mz = off_v + kStages * kSlot;              // stream 1's maximum and sum per row
-  static constexpr uint32_t off_bar = off_mz + kRows * 8;
+  static constexpr uint32_t off_list = off_mz + kRows * 8;                 // the loaders' key positions
+  static constexpr uint32_t off_bar = off_list + kLoadWarps * kKeys * 4;
   static constexpr uint32_t off_tmem = off_bar + 16 * 8;
   static constexpr uint32_t off_work = off_tmem + 16;
-  static constexpr uint32_t bytes = off_work + 32;
+  static constexpr uint32_t bytes = off_work + 48;
   static constexpr uint32_t alloc = bytes + 1024;                          // slack to align the base to 1 KB
 };
 
@@ -106,88 +100,46 @@ __device__ __forceinline__ void regs_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
 }
 
-// What a CTA works on.
-struct Work {
-  int32_t seq;        // -1: nothing
-  int32_t token0;     // first token of the sequence's chunk
-  int32_t row0;       // first row (token x GQA row) of the CTA within the sequence
-  int32_t rows;       // rows of the CTA (1 .. 256)
-  int32_t keys;       // kv_b (within the table)
-  int32_t shift;      // keys before the first token's own: its row sees shift + 1 keys (causal)
-  int32_t key0;       // first key of the CTA's split
-  int32_t tiles;      // key tiles of the CTA
-};
-
-// Resolve blockIdx into a Work, by one converged warp.  The tiles of a sequence
-// are taken from its last (most keys under the causal mask) to its first.
-__device__ __forceinline__ Work find_work(const ChunkParams& p, int tile, int split, int lane) {
-  Work w;
-  w.seq = -1, w.rows = 0, w.tiles = 0;
-  int before = 0;
-  for (int b0 = 0; b0 < p.num_seqs; b0 += 32) {
-    const int b = b0 + lane;
-    int first = 0, n = 0;
-    if (b < p.num_seqs) {
-      first = p.cu[b];
-      const int last = p.cu[b + 1];
-      if (first < 0 || last < first || last > p.num_tokens)
-        set_status(p.status, TA_ERR_BOUNDS);
-      else
-        n = last - first;
-    }
-    const int mine = int((int64_t(n) * p.group + kPairRows - 1) / kPairRows);
-    int upto = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, upto, off);
-      if (lane >= off) upto += t;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, tile < before + upto);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      const int local = tile - before - __shfl_sync(0xffffffffu, upto - mine, src);
-      const int tiles = __shfl_sync(0xffffffffu, mine, src);
-      n = __shfl_sync(0xffffffffu, n, src);
-      w.seq = b0 + src;
-      w.token0 = __shfl_sync(0xffffffffu, first, src);
-      w.row0 = (tiles - 1 - local) * kPairRows;
-      w.rows = min(kPairRows, n * p.group - w.row0);
-      int keys = p.lens[w.seq];
-      const int64_t most = int64_t(p.width) << p.page_shift;
-      if (keys < 0 || keys > most) {
-        set_status(p.status, TA_ERR_BOUNDS);
-        keys = keys < 0 ? 0 : int(most);
-      }
-      w.keys = keys;
-      w.shift = p.causal ? keys - n : INT32_MAX / 2;
-      // keys that the CTA's last row sees
-      const int seen = max(0, min(keys, w.shift + (w.row0 + w.rows - 1) / p.group + 1));
-      const int64_t start = int64_t(split) * p.split_tiles * kKeys;
-      w.key0 = int(min(start, int64_t(seen)));
-      const int end = int(min(start + int64_t(p.split_tiles) * kKeys, int64_t(seen)));
-      w.tiles = (end - w.key0 + kKeys - 1) / kKeys;
-      return w;
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
-  }
-  return w;
-}
-
-// 16 bytes of a key row per lane into a ring slot: warp-wide gather of one tile.
+// Gather one tile into a ring slot, 16 bytes of a row per lane and copy; a
+// position of -1 gives zeros.  `list` (512 bytes of shared memory of this warp)
+// takes the positions round: they come back four rows at a time.  Kept to three
+// instructions a copy (one multiply-add for the source, one add for the slot):
+// the copies of K and V of a tile are on the path from a freed slot to its next
+// use, and both softmax warps of the same scheduler are busy.
 template <int D>
-__device__ __forceinline__ void load_tile(unsigned char* slot, const uint16_t* pool, const int (&pos)[4], int lane) {
+__device__ __forceinline__ void load_tile(uint32_t slot, const uint16_t* pool, const int (&pos)[4], int* list, int lane) {
   constexpr int LPR = D / 8, RPI = 32 / LPR;     // lanes of a row, rows of an instruction
-  const int c = lane % LPR, r = lane / LPR;
+  constexpr int kRun = kKeys / RPI;              // rows of a group of lanes: consecutive
+  const int c = lane % LPR, r = (lane / LPR) * kRun;
+  *reinterpret_cast<int4*>(list + 4 * lane) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+  const bool whole = __all_sync(0xffffffffu, pos[0] >= 0 && pos[1] >= 0 && pos[2] >= 0 && pos[3] >= 0);
+  __syncwarp();
+  const char* src = reinterpret_cast<const char*>(pool) + c * 16;
+  uint32_t dst[8];                               // rows u, u + 8, ... differ by 1 KB
 #pragma unroll
-  for (int i = 0; i < kKeys / RPI; ++i) {
-    const int row = i * RPI + r;
-    const int at = __shfl_sync(0xffffffffu, pos[(i * RPI) / 32], row & 31);
-    cp_async16_zfill(slot + swz<D>(row, c), pool + int64_t(max(at, 0)) * D + c * 8, at >= 0 ? 16u : 0u);
+  for (int u = 0; u < 8; ++u) dst[u] = slot + swz<D>(r + u, c);
+#pragma unroll 2
+  for (int i = 0; i < kRun; i += 8) {
+    const int4 a = *reinterpret_cast<const int4*>(list + r + i), b = *reinterpret_cast<const int4*>(list + r + i + 4);
+    const int at[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (whole) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst[u] + i * 128),
+                     "l"(src + uint64_t(uint32_t(at[u])) * (D * 2)));
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst[u] + i * 128),
+                     "l"(src + uint64_t(uint32_t(max(at[u], 0))) * (D * 2)), "r"(at[u] >= 0 ? 16u : 0u));
+    }
   }
+  __syncwarp();
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1) chunk_kernel(ChunkParams p) {
+__global__ void __launch_bounds__(kThreads, 1)
+    chunk_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ ChunkMaps maps) {
   using S = Smem<D>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -196,27 +148,27 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(ChunkParams p) {
   Work* work = reinterpret_cast<Work*>(smem + S::off_work);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int head = blockIdx.y, split = blockIdx.z;
+  const int split = blockIdx.y;
   const int G = p.group;
 
   if (warp == 0) {
-    const Work w = find_work(p, blockIdx.x, split, lane);
-    if (lane == 0) {
-      *work = w;
-      const int rows_b = max(0, w.rows - kRows);
-      for (int s = 0; s < 2; ++s) {
-        mbar_init(&bars[K_FULL + s], 1);
-        mbar_init(&bars[K_EMPTY + s], 1);
-        mbar_init(&bars[V_FULL + s], 1);
-        mbar_init(&bars[V_EMPTY + s], 1);
-        mbar_init(&bars[S_FULL + s], 1);
-        // softmax warps with rows: those without take no part
-        const int rows_t = (s == 0 || rows_b == 0) ? min(kRows, max(1, w.rows)) : rows_b;
-        mbar_init(&bars[P_FULL + s], (rows_t + 31) / 32);
-        mbar_init(&bars[Q_FULL + s], (rows_t + 31) / 32);
-        mbar_init(&bars[PV_DONE + s], 1);
-      }
-      fence_barrier_init();
+    const Work found = find_work<kPairRows>(p, blockIdx.x, split, lane);
+    if (lane == 0) *work = found;
+  } else if (tid == 32) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars[K_FULL + s], 1);
+      mbar_init(&bars[K_EMPTY + s], 1);
+      mbar_init(&bars[V_FULL + s], 1);
+      mbar_init(&bars[V_EMPTY + s], 1);
+      mbar_init(&bars[S_FULL + s], 1);
+      mbar_init(&bars[P_FULL + s], 4);
+      mbar_init(&bars[PV_DONE + s], 1);
+      mbar_init(&bars[Q_FULL + s], 4);
+    }
+    fence_barrier_init();
+    if (p.box_rows) {
+      prefetch_tensormap(&maps.k);
+      prefetch_tensormap(&maps.v);
     }
   } else if (warp == kIssueWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
@@ -229,45 +181,79 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(ChunkParams p) {
   tc_fence_after();
   pdl_trigger();                                 // the merge may be placed; it waits for this grid's end
   const uint32_t tmem = *tmem_slot;
-  const Work w = *work;
-  const int ntiles = w.seq < 0 ? 0 : w.tiles;
+  const Work& w = *work;
+  const int ntiles = w.seq < 0 ? 0 : (w.count + kKeys - 1) / kKeys;
   const bool two = w.rows > kRows;               // two row tiles, else two key streams
   bool alive = true;
 
   if (warp < kLoadWarps) {
     regs_down<kOtherRegs>();
-    // ---------------- K/V gather ----------------
+    // ---------------- K/V tiles ----------------
     const bool is_k = warp < 2;
     const int slot = warp & 1;
     unsigned char* dst = smem + (is_k ? S::off_k : S::off_v) + slot * S::kSlot;
-    const uint16_t* pool = (is_k ? p.k : p.v) + int64_t(head) * p.pool_tokens * D;
     uint64_t* full = &bars[(is_k ? K_FULL : V_FULL) + slot];
     uint64_t* empty = &bars[(is_k ? K_EMPTY : V_EMPTY) + slot];
+    const int page = 1 << p.page_shift, box = p.box_rows;
+    int* list = reinterpret_cast<int*>(smem + S::off_list) + warp * kKeys;
+    const int head = w.head, keys = w.keys;
+    const uint16_t* pool = (is_k ? p.k : p.v) + int64_t(head) * p.pool_tokens * D;
     const int32_t* table = p.table + int64_t(max(w.seq, 0)) * p.table_stride;
+    int last = -1;
     for (int j = slot; j < ntiles; j += 2) {
+      const int key0 = w.key0 + j * kKeys;
+      // A whole tile of pages of 16 and more comes in boxes of a page's rows,
+      // one of smaller pages in one box where its positions follow one another
+      // (those of a tree node do); anything else is gathered row by row.
+      bool boxes = box > 0 && key0 + kKeys <= keys;
       int pos[4];
-      bool bad = false;
+      if (boxes && page >= box) {
+        const int key = key0 + min(lane, kKeys / box - 1) * box;
+        const int64_t at = int64_t(table[key >> p.page_shift]) * page + (key & (page - 1));
+        boxes = __all_sync(0xffffffffu, at >= 0 && at + box <= p.pool_tokens);
+        pos[0] = int(at);
+      }
+      if (!boxes || page < box) {
+        // positions of keys 4 lane .. 4 lane + 3; -1 past the keys or outside the pools
+        int entry[4];
+        bool bad = false;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = w.key0 + j * kKeys + i * 32 + lane;
-        pos[i] = -1;
-        if (key < w.keys) {
-          const int page = 1 << p.page_shift;
-          const int64_t at = int64_t(table[key >> p.page_shift]) * page + (key & (page - 1));
-          if (at >= 0 && at < p.pool_tokens)
-            pos[i] = int(at);
-          else
-            bad = true;
+        for (int i = 0; i < 4; ++i) entry[i] = table[min(key0 + 4 * lane + i, keys - 1) >> p.page_shift];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + 4 * lane + i;
+          const int64_t at = int64_t(entry[i]) * page + (key & (page - 1));
+          const bool inside = at >= 0 && at < p.pool_tokens;
+          bad |= key < keys && !inside;
+          pos[i] = key < keys && inside ? int(at) : -1;
+        }
+        if (bad) set_status(p.status, TA_ERR_BOUNDS);
+        if (boxes) {
+          const int first = __shfl_sync(0xffffffffu, pos[0], 0) + 4 * lane;
+          boxes = __all_sync(0xffffffffu, pos[0] >= 0 && pos[0] == first && pos[1] == first + 1 &&
+                                              pos[2] == first + 2 && pos[3] == first + 3);
         }
       }
-      if (bad) set_status(p.status, TA_ERR_BOUNDS);
       if (j >= kStages && !warp_wait(empty, (j / kStages + 1) & 1, p.status)) break;
-      load_tile<D>(dst, pool, pos, lane);
-      cp_async_wait_all();
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(full);
+      if (boxes) {
+        if (lane == 0) mbar_arrive_expect_tx(full, S::kTile);
+        __syncwarp();
+        if (lane < kKeys / box) {
+#pragma unroll
+          for (int h = 0; h < D / 64; ++h)
+            tma_load_3d(dst + h * S::kBlock + lane * box * 128, is_k ? &maps.k : &maps.v, h * 64, pos[0], head, full);
+        }
+      } else {
+        load_tile<D>(smem_u32(dst), pool, pos, list, lane);
+        cp_async_wait_all();
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full);
+      }
+      last = j;
     }
+    // no copy of this warp may land after the CTA's shared memory is released
+    if (last >= 0) warp_wait(full, (last / kStages) & 1, p.status);
   } else if (warp < kSoftmaxWarp0) {
     regs_down<kOtherRegs>();
     if (warp == kIssueWarp && ntiles > 0) {
@@ -303,29 +289,35 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(ChunkParams p) {
         if (!two || t == 1) umma_commit_warp(&bars[V_EMPTY + j % kStages]);
       };
       auto full = [&](int bar, int j) { return warp_wait(&bars[bar + j % kStages], (j / kStages) & 1, p.status); };
+      // V of step (t, u) and the K that follows it: waited for while the
+      // softmax of the step still runs, so that P's arrival is followed by
+      // MMAs only (a wait on a completed barrier costs about 150 cycles)
+      auto inputs = [&](int t, int u) {
+        if (two && t == 1) return true;                      // stream 0's step has waited for the same tiles
+        return full(V_FULL, tile_of(t, u)) && (u + 1 >= count[t] || full(K_FULL, tile_of(t, u + 1)));
+      };
 
       for (int t = 0; t < 2 && alive; ++t) {
         if (count[t] == 0) continue;
-        const int j = tile_of(t, 0);
-        if (!warp_wait(&bars[Q_FULL + (two ? t : 0)], 0, p.status) || !full(K_FULL, j)) { alive = false; break; }
+        if (!warp_wait(&bars[Q_FULL + (two ? t : 0)], 0, p.status) || !full(K_FULL, tile_of(t, 0))) {
+          alive = false;
+          break;
+        }
         tc_fence_after();
-        issue_s(t, j);
+        issue_s(t, tile_of(t, 0));
       }
+      if (alive && !inputs(0, 0)) alive = false;
       for (int u = 0; u < count[0] && alive; ++u) {
         for (int t = 0; t < 2; ++t) {
           if (u >= count[t]) continue;
-          const int j = tile_of(t, u), next = tile_of(t, u + 1);
-          const bool more = u + 1 < count[t];
-          // V(j) and the next K are normally there before P(u): wait for them
-          // first, so that P's arrival is followed by MMAs only
-          if (!full(V_FULL, j) || (more && !full(K_FULL, next)) ||
-              !warp_wait(&bars[P_FULL + t], u & 1, p.status)) {
-            alive = false;
-            break;
-          }
+          if (!warp_wait(&bars[P_FULL + t], u & 1, p.status)) { alive = false; break; }
           tc_fence_after();
-          issue_pv(t, u, j);
-          if (more) issue_s(t, next);
+          issue_pv(t, u, tile_of(t, u));
+          if (u + 1 < count[t]) issue_s(t, tile_of(t, u + 1));
+          // the next step's inputs
+          const bool other = t == 0 && u < count[1];
+          const int nt = other ? 1 : 0, nu = other ? u : u + 1;
+          if (nu < count[nt] && !inputs(nt, nu)) { alive = false; break; }
         }
       }
       // the last commits must land before the CTA's shared memory is released
@@ -340,38 +332,44 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(ChunkParams p) {
     // ---------------- softmax and epilogue ----------------
     const int t = (warp - kSoftmaxWarp0) >> 2;
     const int quad = warp & 3;
-    const int row = quad * 32 + lane;                       // row within the tile, its TMEM lane
-    const int trow = (two ? t * kRows : 0) + row;           // row within the CTA
-    const int base_row = (two ? t * kRows : 0) + quad * 32; // first row of the warp
-    const bool active = w.seq >= 0 && base_row < w.rows;    // uniform in the warp
-    if (active) {
-      const bool mine = trow < w.rows;
-      const int local = w.row0 + trow;                      // row within the sequence
-      const int token = w.token0 + (mine ? local / G : 0), g = mine ? local % G : 0;
-      const int hq = head * G + g;
-      const int limit = mine ? min(w.keys, w.shift + local / G + 1) - w.key0 : 0;   // visible keys of the split
-      const int count = two ? ntiles : (ntiles + 1 - t) / 2;
-      const uint32_t lane_addr = tmem + (uint32_t(quad * 32) << 16);
-      const uint32_t s_col = kColS + t * 128, o_col = kColO + t * 128;
+    const int row = quad * 32 + lane;                         // row within the tile, its TMEM lane
+    const uint32_t lane_addr = tmem + (uint32_t(quad * 32) << 16);
+    const uint32_t s_col = kColS + t * 128, o_col = kColO + t * 128;
+    const float scale = p.scale_log2;
+    const int trow = (two ? t * kRows : 0) + row;             // row within the CTA
+    const bool active = w.seq >= 0 && (two ? t * kRows : 0) + quad * 32 < w.rows;   // uniform in the warp
+    const bool mine = w.seq >= 0 && trow < w.rows;
+    const int count = two ? ntiles : (ntiles + 1 - t) / 2;
+    const bool joined = !two && ntiles > 1;                   // two key streams of the same rows
+    {
+      const int local = mine ? w.row0 + trow : 0;             // row within the sequence
+      const int token = w.token0 + local / G, hq = w.head * G + local % G;
+      // visible keys of this row from the stream's first tile on
+      const int limit = mine ? min(w.keys, w.shift + local / G + 1) - w.key0 - (two ? 0 : t * kKeys) : 0;
 
-      if (ntiles > 0 && (two || t == 0)) {
+      if (ntiles > 0 && (two || t == 0)) {                    // the row's query, K-major with the swizzle
         unsigned char* qs = smem + S::off_q + (two ? t : 0) * S::kSlot;
         const uint4* src = reinterpret_cast<const uint4*>(p.q + int64_t(token) * p.q_st + int64_t(hq) * p.q_sh);
-        uint4 x[D / 8];
+        if (mine) {
+          uint4 x[D / 8];
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) x[c] = mine ? src[c] : make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < D / 8; ++c) x[c] = src[c];
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(qs + swz<D>(row, c)) = x[c];
+          for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(qs + swz<D>(row, c)) = x[c];
+        }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[Q_FULL + (two ? t : 0)]);
       }
 
-      const float scale = p.scale_log2;
       float m_run = -INFINITY, z = 0.f;
       for (int u = 0; u < count; ++u) {
-        const int valid = limit - (two ? u : 2 * u + t) * kKeys;     // visible keys of this tile and after
         if (!warp_wait(&bars[S_FULL + t], u & 1, p.status)) { alive = false; break; }
+        if (!active) {                                        // no rows: P's lanes may hold anything
+          if (lane == 0) mbar_arrive(&bars[P_FULL + t]);
+          continue;
+        }
+        const int valid = limit - u * (two ? kKeys : 2 * kKeys);      // visible keys of this tile and after
         tc_fence_after();
         float s[kKeys];
         {
@@ -437,91 +435,69 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(ChunkParams p) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[P_FULL + t]);
       }
-      if (count > 0 && alive && !warp_wait(&bars[PV_DONE + t], 0, p.status)) alive = false;
+
+      // O_t is complete (stream 0 of joined streams reads both)
+      if (alive && count > 0 && !warp_wait(&bars[PV_DONE + t], 0, p.status)) alive = false;
+      if (alive && joined && t == 0 && !warp_wait(&bars[PV_DONE + 1], 0, p.status)) alive = false;
       tc_fence_after();
       if (!alive) z = 0.f;
 
-      // two key streams: stream 1 hands its O, maximum and sum to stream 0
       float m = m_run, scale_a = 1.f, scale_b = 0.f;
-      // its O goes where only its own MMAs read, columns halved over the second
-      // query slot (not used here) and K slot 1 (the tiles of odd parity)
-      auto other = [&](int chunk) {                         // 4 columns of this row
-        unsigned char* half = smem + (chunk < D / 8 ? S::off_q : S::off_k) + S::kSlot;
-        constexpr int kSwz = (D / 8 < 8 ? D / 8 : 8) - 1;
-        return reinterpret_cast<float4*>(half) + row * (D / 8) + ((chunk % (D / 8)) ^ (row & kSwz));
-      };
-      float2* mz = reinterpret_cast<float2*>(smem + S::off_mz) + row;
-      const bool joined = !two && ntiles > 1;
-      const int warps = (w.rows + 31) / 32;                 // active warps of a stream (two key streams)
-      if (joined && t == 1) {
+      if (joined && active) {
+        float2* mz = reinterpret_cast<float2*>(smem + S::off_mz) + row;
+        if (t == 1) *mz = make_float2(m_run, z);
+        named_sync(1, 2 * 32 * ((w.rows + 31) / 32));         // the active warps of both streams
+        const float2 b = *mz;
+        m = fmaxf(m_run, b.x);
+        const float m_use = m == -INFINITY ? 0.f : m;
+        scale_a = fast_exp2(m_run - m_use);
+        scale_b = b.y > 0.f ? fast_exp2(b.x - m_use) : 0.f;
+        z = z * scale_a + b.y * scale_b;
+      }
+      if (active && (two || t == 0)) {
+      const float inv = z > 0.f ? 1.f / z : 0.f;
+      scale_a = z > 0.f ? scale_a * inv : 0.f;
+      scale_b *= inv;
+      const int64_t index = int64_t(token) * p.hq + hq;
+      const float lse = z > 0.f ? (m + fast_log2(z)) * kLn2 : -INFINITY;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32(lane_addr + o_col + c * 32, o);
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        float y[32];
+        if (ntiles > 0) {
+          tmem_ld32(lane_addr + kColO + (two ? t * 128 : 0) + c * 32, o);
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) y[i] = scale_a > 0.f ? __uint_as_float(o[i]) * scale_a : 0.f;
+        if (joined) {
+          tmem_ld32(lane_addr + kColO + 128 + c * 32, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *other(c * 8 + i) =
-                make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
-                            __uint_as_float(o[4 * i + 3]));
+          for (int i = 0; i < 32; ++i) y[i] += scale_b > 0.f ? __uint_as_float(o[i]) * scale_b : 0.f;
         }
-        *mz = make_float2(m_run, z);
+        if (!mine) continue;
+        if (p.splits > 1) {
+          if (!(z > 0.f)) continue;                           // no weight in the merge: not read
+          float* dst = p.part + (int64_t(split) * p.num_tokens * p.hq + index) * D + c * 32;
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(dst + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+        } else {
+          uint16_t* dst = p.out + index * D + c * 32;
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            *reinterpret_cast<uint4*>(dst + i) =
+                make_uint4(Elem<T>::pack2(y[i], y[i + 1]), Elem<T>::pack2(y[i + 2], y[i + 3]),
+                           Elem<T>::pack2(y[i + 4], y[i + 5]), Elem<T>::pack2(y[i + 6], y[i + 7]));
+        }
       }
-      if (joined) named_sync(1, warps * 2 * 32);
-      if (two || t == 0) {
-        if (joined) {
-          const float2 b = *mz;
-          m = fmaxf(m_run, b.x);
-          const float m_use = m == -INFINITY ? 0.f : m;
-          scale_a = fast_exp2(m_run - m_use);
-          scale_b = b.y > 0.f ? fast_exp2(b.x - m_use) : 0.f;
-          z = z * scale_a + b.y * scale_b;
-        }
-        const float inv = z > 0.f ? 1.f / z : 0.f;
-        scale_a = z > 0.f ? scale_a * inv : 0.f;
-        scale_b *= inv;
-        const int64_t index = int64_t(token) * p.hq + hq;
-        const float lse = z > 0.f ? (m + fast_log2(z)) * kLn2 : -INFINITY;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          float y[32];
-          if (ntiles > 0) {
-            tmem_ld32(lane_addr + o_col + c * 32, o);
-            tmem_wait_ld();
-          }
-#pragma unroll
-          for (int i = 0; i < 32; ++i) y[i] = scale_a > 0.f ? __uint_as_float(o[i]) * scale_a : 0.f;
-          if (joined && scale_b > 0.f) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 b = *other(c * 8 + i);
-              y[4 * i] += b.x * scale_b, y[4 * i + 1] += b.y * scale_b;
-              y[4 * i + 2] += b.z * scale_b, y[4 * i + 3] += b.w * scale_b;
-            }
-          }
-          if (!mine) continue;
-          if (p.splits > 1) {
-            if (!(z > 0.f)) continue;                       // no weight in the merge: not read
-            float* dst = p.part + (int64_t(split) * p.num_tokens * p.hq + index) * D + c * 32;
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(dst + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
-          } else {
-            uint16_t* dst = p.out + index * D + c * 32;
-#pragma unroll
-            for (int i = 0; i < 32; i += 8)
-              *reinterpret_cast<uint4*>(dst + i) =
-                  make_uint4(Elem<T>::pack2(y[i], y[i + 1]), Elem<T>::pack2(y[i + 2], y[i + 3]),
-                             Elem<T>::pack2(y[i + 4], y[i + 5]), Elem<T>::pack2(y[i + 6], y[i + 7]));
-          }
-        }
-        if (mine) {
-          if (p.splits > 1)
-            p.part_lse[int64_t(split) * p.num_tokens * p.hq + index] = lse;
-          else if (p.lse)
-            p.lse[index] = lse;
-        }
+      if (mine) {
+        if (p.splits > 1)
+          p.part_lse[int64_t(split) * p.num_tokens * p.hq + index] = lse;
+        else if (p.lse)
+          p.lse[index] = lse;
+      }
       }
     }
   }
@@ -548,6 +524,32 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(ChunkPara
   pdl_wait();
   const int token = int(index / p.hq);
   if (index >= rows || token < first || token >= last) return;
+  const float* rows_in = p.part + index * D + lane * E;
+  // the first eight rows come in beside their LSEs; rows without weight were
+  // not written and are dropped by a select
+  constexpr int kAhead = 8;
+  float x[kAhead][E];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[i][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (s0 + i >= p.splits) break;
+      const float* src = rows_in + int64_t(s0 + i) * rows * D;
+      if constexpr (E == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src);
+        x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
+      } else if constexpr (E == 2) {
+        const float2 v = *reinterpret_cast<const float2*>(src);
+        x[i][0] = v.x, x[i][1] = v.y;
+      } else {
+        x[i][0] = *src;
+      }
+    }
+  };
+  load(0);
   float l0 = lane < p.splits ? p.part_lse[lane * rows + index] : -INFINITY;
   float l1 = lane + 32 < p.splits ? p.part_lse[(lane + 32) * rows + index] : -INFINITY;
   const float m = warp_max(fmaxf(l0, l1));
@@ -558,25 +560,24 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(ChunkPara
   float acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int s0 = 0; s0 < p.splits; s0 += 8) {
-    float x[8][E];
+  for (int s0 = 0; s0 < p.splits; s0 += kAhead) {
+    if (s0 > 0) load(s0);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int s = s0 + i;
-      const float weight = s < p.splits ? __shfl_sync(0xffffffffu, s < 32 ? l0 : l1, s & 31) : 0.f;
-      const float* src = p.part + (int64_t(s) * rows + index) * D + lane * E;
+    for (int i = 0; i < kAhead; ++i) {
+      const float weight = __shfl_sync(0xffffffffu, s0 + i < 32 ? l0 : l1, (s0 + i) & 31);
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[i][e] = weight > 0.f ? src[e] * weight : 0.f;
+      for (int e = 0; e < E; ++e) acc[e] += weight > 0.f ? x[i][e] * weight : 0.f;
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += x[i][e];
   }
   const float inv = z > 0.f ? 1.f / z : 0.f;
   uint16_t* dst = p.out + index * D + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; ++e) dst[e] = Elem<T>::from_float(acc[e] * inv);
+  if constexpr (E == 4)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack2(acc[0] * inv, acc[1] * inv),
+                                                Elem<T>::pack2(acc[2] * inv, acc[3] * inv));
+  else if constexpr (E == 2)
+    *reinterpret_cast<uint32_t*>(dst) = Elem<T>::pack2(acc[0] * inv, acc[1] * inv);
+  else
+    *dst = Elem<T>::from_float(acc[0] * inv);
   if (lane == 0 && p.lse) p.lse[index] = z > 0.f ? m + logf(z) : -INFINITY;
 }
 
@@ -603,40 +604,64 @@ int sm_count() {
   return sms;
 }
 
-// Most row tiles a batch of num_tokens over num_seqs sequences can have.
-int64_t tile_bound(int64_t tokens, int64_t seqs, int64_t group) {
-  return tokens * group / kPairRows + std::min(tokens, seqs);
-}
+// Which kernel runs and how the keys are cut, from sizes known on the host.
+struct Plan {
+  bool small;          // the small-row kernel
+  int64_t tiles;       // row tiles that the batch can have at most
+  int splits;
+  int split_keys;
+};
 
-// Splits of the keys: the least modelled time (tenths of a microsecond) of the
-// waves of CTAs, a CTA costing kFixed plus kPerTile a key tile, and the merge.
-Split choose_split(int64_t tokens, int64_t seqs, int64_t group, int64_t hk, int64_t most_keys, int sms) {
-  constexpr int64_t kFixed = 50, kPerTile = 10, kMerge = 35;
-  const int64_t base = tile_bound(tokens, seqs, group) * hk;
-  const int64_t tiles = std::max<int64_t>(1, (most_keys + kKeys - 1) / kKeys);
-  Split best{1, int(std::min<int64_t>(tiles, INT32_MAX / kKeys))};
+// Batches of at most kSmallRows rows a sequence on average run on the small-row
+// kernel, others on the tensor-core tiles.  The keys are cut where that lowers
+// a modelled time (tenths of a microsecond; measured on one B200): the waves of
+// CTAs, each kFixed plus kPerStep a step of keys, and the merge of the splits,
+// kMerge plus its bytes at 3 TB/s.
+Plan choose_plan(int64_t tokens, int64_t seqs, int64_t group, int64_t hk, int64_t dim, int64_t most_keys, int sms) {
+  Plan plan{};
+  plan.small = tokens * group <= kSmallRows * seqs;
+  const int64_t rows = plan.small ? kSmallRows : kPairRows;
+  plan.tiles = tokens * group / rows + std::min(tokens, seqs);
+  const int64_t step = plan.small ? kSmallKeys : kKeys, slots = plan.small ? kSmallCtas * sms : sms;
+  const int64_t kFixed = plan.small ? 30 : 45, kPerStep = plan.small ? 12 : 10, kMerge = 25;
+  const int64_t base = plan.tiles * hk, steps = std::max<int64_t>(1, (most_keys + step - 1) / step);
   int64_t least = INT64_MAX;
-  for (int64_t s = 1; s <= std::min<int64_t>(kMaxSplits, tiles); ++s) {
-    const int64_t per = (tiles + s - 1) / s;
-    if (s > 1 && (tiles + per - 1) / per != s) continue;     // the same cut as a smaller s
-    const int64_t waves = (base * s + sms - 1) / sms;
-    const int64_t cost = waves * (kFixed + per * kPerTile) + (s > 1 ? kMerge : 0);
+  for (int64_t s = 1; s <= std::min<int64_t>(kMaxSplits, steps); ++s) {
+    const int64_t per = (steps + s - 1) / s;
+    if (s > 1 && (steps + per - 1) / per != s) continue;     // the same cut as a smaller s
+    const int64_t waves = (base * s + slots - 1) / slots;
+    int64_t cost = waves * (kFixed + per * kPerStep);
+    if (s > 1) cost += kMerge + s * tokens * group * hk * (dim + 1) * 8 / 300000;
     if (cost < least) {
       least = cost;
-      best.splits = int(s);
-      best.tiles = int(per);
+      plan.splits = int(s);
+      plan.split_keys = int(std::min<int64_t>(per * step, INT32_MAX));
     }
-    if (s > 1 && waves > 8) break;
+    if (s > 1 && waves > 16) break;
   }
-  return best;
+  return plan;
 }
 
 int64_t partial_bytes(int splits, int64_t tokens, int64_t hq, int64_t dim) {
   return splits > 1 ? int64_t(splits) * tokens * hq * (dim + 1) * 4 : 0;
 }
 
+// A pool [heads, tokens, D] as boxes of 64 columns x `rows` tokens, 128-byte swizzle.
+template <int D>
+bool make_chunk_map(CUtensorMap* map, const void* base, int64_t tokens, int heads, int rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn || tokens <= 0) return false;
+  cuuint64_t dims[3] = {D, cuuint64_t(tokens), cuuint64_t(heads)};
+  cuuint64_t strides[2] = {D * 2, cuuint64_t(tokens) * D * 2};
+  cuuint32_t box[3] = {64, cuuint32_t(rows), 1};
+  cuuint32_t elem[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, elem,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D>
-cudaError_t launch_typed(const ChunkParams& p, int64_t tiles, int hk, cudaStream_t stream) {
+cudaError_t launch_typed(ChunkParams p, int64_t tiles, cudaStream_t stream) {
   auto kernel = chunk_kernel<T, D>;
   static std::atomic<uint64_t> configured{0};                // one bit a device
   int dev = 0;
@@ -647,19 +672,30 @@ cudaError_t launch_typed(const ChunkParams& p, int64_t tiles, int hk, cudaStream
     if (err != cudaSuccess) return err;
     if (dev < 64) configured.fetch_or(uint64_t(1) << dev);
   }
-  kernel<<<dim3(unsigned(tiles), unsigned(hk), unsigned(p.splits)), kThreads, Smem<D>::alloc, stream>>>(p);
-  err = cudaGetLastError();
-  if (err != cudaSuccess || p.splits == 1) return err;
-  const int64_t rows = int64_t(p.num_tokens) * p.hq;
-  return launch_dependent(chunk_merge_kernel<T, D>, dim3(unsigned((rows + kMergeWarps - 1) / kMergeWarps)),
-                          dim3(kMergeWarps * 32), 0, stream, p);
+  ChunkMaps maps{};
+  const int page = 1 << p.page_shift;
+  const int rows = page < 16 ? kKeys : std::min(page, kKeys);
+  if (D >= 64 && make_chunk_map<D>(&maps.k, p.k, p.pool_tokens, p.hk, rows) &&
+      make_chunk_map<D>(&maps.v, p.v, p.pool_tokens, p.hk, rows))
+    p.box_rows = rows;
+  kernel<<<dim3(unsigned(tiles * p.hk), unsigned(p.splits)), kThreads, Smem<D>::alloc, stream>>>(p, maps);
+  return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t launch_dim(const ChunkParams& p, int64_t tiles, int hk, int head_dim, cudaStream_t stream) {
-  if (head_dim == 128) return launch_typed<T, 128>(p, tiles, hk, stream);
-  if (head_dim == 64) return launch_typed<T, 64>(p, tiles, hk, stream);
-  return launch_typed<T, 32>(p, tiles, hk, stream);
+cudaError_t launch_chunk_merge(const ChunkParams& p, int head_dim, cudaStream_t stream) {
+  const int64_t rows = int64_t(p.num_tokens) * p.hq;
+  const dim3 grid{unsigned((rows + kMergeWarps - 1) / kMergeWarps)}, block{kMergeWarps * 32};
+  if (head_dim == 128) return launch_dependent(chunk_merge_kernel<T, 128>, grid, block, 0, stream, p);
+  if (head_dim == 64) return launch_dependent(chunk_merge_kernel<T, 64>, grid, block, 0, stream, p);
+  return launch_dependent(chunk_merge_kernel<T, 32>, grid, block, 0, stream, p);
+}
+
+template <typename T>
+cudaError_t launch_dim(const ChunkParams& p, int64_t tiles, int head_dim, cudaStream_t stream) {
+  if (head_dim == 128) return launch_typed<T, 128>(p, tiles, stream);
+  if (head_dim == 64) return launch_typed<T, 64>(p, tiles, stream);
+  return launch_typed<T, 32>(p, tiles, stream);
 }
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -675,9 +711,9 @@ extern "C" int64_t ta_chunk_workspace_bytes(int32_t num_tokens, int32_t num_seqs
   if (num_tokens <= 0 || num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads ||
       head_dim <= 0 || table_width < 0 || page_size <= 0)
     return 0;
-  const Split s = choose_split(num_tokens, num_seqs, num_q_heads / num_kv_heads, num_kv_heads,
-                               int64_t(table_width) * page_size, sm_count());
-  return partial_bytes(s.splits, num_tokens, num_q_heads, head_dim);
+  const Plan plan = choose_plan(num_tokens, num_seqs, num_q_heads / num_kv_heads, num_kv_heads, head_dim,
+                                int64_t(table_width) * page_size, sm_count());
+  return partial_bytes(plan.splits, num_tokens, num_q_heads, head_dim);
 }
 
 extern "C" int ta_chunk_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* kpool,
@@ -699,15 +735,15 @@ extern "C" int ta_chunk_attention(const void* q, int64_t q_stride_token, int64_t
   const int64_t most_keys = int64_t(table_width) * page_size;
   const int group = num_q_heads / num_kv_heads;
   if (most_keys > INT32_MAX / 4 || pool_tokens > INT32_MAX || int64_t(num_tokens) * group > INT32_MAX / 2 ||
-      int64_t(num_tokens) > INT32_MAX / 4 || num_kv_heads > 65535)
+      int64_t(num_tokens) > INT32_MAX / 4)
     return TA_ERR_UNSUPPORTED;
+  const Plan plan = choose_plan(num_tokens, num_seqs, group, num_kv_heads, head_dim, most_keys, sm_count());
+  if (plan.tiles * num_kv_heads > INT32_MAX) return TA_ERR_UNSUPPORTED;
   if (!q || !kpool || !vpool || !kv_lens || !cu_q || !out || (table_width > 0 && !table)) return TA_ERR_ARG;
   if (!aligned(q) || !aligned(kpool) || !aligned(vpool) || !aligned(out) || q_stride_token < 0 || q_stride_head < 0 ||
       (q_stride_token & 7) || (q_stride_head & 7))
     return TA_ERR_ARG;
-  const int64_t tiles = tile_bound(num_tokens, num_seqs, group);
-  const Split s = choose_split(num_tokens, num_seqs, group, num_kv_heads, most_keys, sm_count());
-  const int64_t need = partial_bytes(s.splits, num_tokens, num_q_heads, head_dim);
+  const int64_t need = partial_bytes(plan.splits, num_tokens, num_q_heads, head_dim);
   if (need > 0 && (!workspace || !aligned(workspace))) return TA_ERR_ARG;
   if (workspace_bytes < need) return TA_ERR_TOO_LARGE;
   ChunkParams p{};
@@ -720,16 +756,23 @@ extern "C" int ta_chunk_attention(const void* q, int64_t q_stride_token, int64_t
   while ((1 << p.page_shift) < page_size) ++p.page_shift;
   p.lens = kv_lens, p.cu = cu_q;
   p.num_seqs = num_seqs, p.num_tokens = num_tokens;
-  p.hq = num_q_heads, p.group = group;
+  p.hq = num_q_heads, p.hk = num_kv_heads, p.group = group;
   p.causal = causal != 0;
   p.out = static_cast<uint16_t*>(out), p.lse = out_lse;
-  p.splits = s.splits, p.split_tiles = s.tiles;
+  p.splits = plan.splits, p.split_keys = plan.split_keys;
   p.part = static_cast<float*>(workspace);
-  p.part_lse = p.part + int64_t(s.splits) * num_tokens * num_q_heads * head_dim;
+  p.part_lse = p.part + int64_t(plan.splits) * num_tokens * num_q_heads * head_dim;
   p.status = status;
   p.scale_log2 = scale * kLog2e;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t err = dtype == TA_DTYPE_BF16 ? launch_dim<__nv_bfloat16>(p, tiles, num_kv_heads, head_dim, st)
-                                                 : launch_dim<__half>(p, tiles, num_kv_heads, head_dim, st);
+  cudaError_t err;
+  if (plan.small)
+    err = launch_chunk_rows(p, plan.tiles, head_dim, dtype, st);
+  else
+    err = dtype == TA_DTYPE_BF16 ? launch_dim<__nv_bfloat16>(p, plan.tiles, head_dim, st)
+                                 : launch_dim<__half>(p, plan.tiles, head_dim, st);
+  if (err == cudaSuccess && plan.splits > 1)
+    err = dtype == TA_DTYPE_BF16 ? launch_chunk_merge<__nv_bfloat16>(p, head_dim, st)
+                                 : launch_chunk_merge<__half>(p, head_dim, st);
   return err == cudaSuccess ? TA_OK : TA_ERR_LAUNCH;
 }

@@ -1,0 +1,324 @@
+// Chunk attention for few query rows a sequence: single tokens of a decode step,
+// a handful of draft tokens (rows = token x GQA row, 16 a CTA).
+//
+// The same rows, keys and result as chunk.cu.  Every key is read once for at
+// most 16 rows, 64 FLOP a byte at D = 128, so HBM bounds it and the 128-row
+// tiles of tcgen05 would stand nearly empty; the work goes through mma.sync
+// m16n8k16 instead, whose 16 rows fit, from shared memory that each warp fills
+// for itself:
+//
+//   a warp takes every fourth block of 16 keys of the CTA's split, K and V rows
+//   gathered by 16-byte cp.async (any page size) into its own ring of kStages
+//   blocks, its page entries read two blocks ahead; no barrier but __syncwarp;
+//   S = Q K^T by 16 mma (Q held in registers), an online softmax with the row
+//   maximum over the quad's lanes, O += P V by 16 mma with P straight from the
+//   S accumulators.  O is rescaled when a maximum grows by more than 2^8.
+//   At the end the four warps' maxima, sums and O meet in shared memory.
+//
+// Two CTAs an SM keep 128 KB of loads in flight at D = 128.
+#include <algorithm>
+#include <atomic>
+
+#include "chunk_common.cuh"
+#include "ta_kernels.cuh"
+#include "tc_common.cuh"
+
+namespace ta {
+
+namespace {
+
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kBlock = 16;                    // keys of a block
+constexpr int kStages = 3;
+constexpr float kRescaleThreshold = 8.f;      // log2 units
+
+static_assert(kSmallKeys == kWarps * kBlock, "a step of the CTA is one block a warp");
+
+template <int D>
+struct RowsSmem {
+  static constexpr int kRow = D * 2;                           // bytes
+  static constexpr int kTile = kBlock * kRow;                  // K or V of a block
+  static constexpr int kWarp = kStages * 2 * kTile;            // ring of a warp
+  static constexpr int kCombine = kSmallRows * D * 4;          // O of a warp at the end
+  static constexpr int kArea = kWarp > kCombine ? kWarp : kCombine;
+  static constexpr int bytes = kWarps * kArea;
+};
+
+// Byte offset of 16-byte chunk c of row r: the chunks of a row are permuted so
+// that the eight rows of an 8 x 8 matrix lie in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t place(int r, int c) {
+  if constexpr (D >= 64)
+    return uint32_t(r * (D * 2) + ((c ^ (r & 7)) << 4));
+  else
+    return uint32_t(r * (D * 2) + ((c ^ ((r >> 1) & 3)) << 4));
+}
+
+__device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (Elem<T>::kCode == TA_DTYPE_BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+        "%2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+        "%2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, kSmallCtas) chunk_rows_kernel(const __grid_constant__ ChunkParams p) {
+  using S = RowsSmem<D>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float s_m[kWarps][kSmallRows], s_z[kWarps][kSmallRows];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int split = blockIdx.y, G = p.group;
+  pdl_trigger();                                 // the merge may be placed; it waits for this grid's end
+  const Work w = find_work<kSmallRows>(p, blockIdx.x, split, lane);   // every warp for itself
+  if (w.seq < 0) return;
+  if (w.count == 0 && p.splits > 1) {            // a split behind the keys: nothing to merge
+    if (tid < w.rows) {
+      const int local = w.row0 + tid;
+      p.part_lse[(int64_t(split) * p.num_tokens + w.token0 + local / G) * p.hq + w.head * G + local % G] = -INFINITY;
+    }
+    return;
+  }
+
+  const int64_t pool = int64_t(w.head) * p.pool_tokens * D;
+  const int32_t* table = p.table + int64_t(w.seq) * p.table_stride;
+  const int page = 1 << p.page_shift;
+  unsigned char* area = smem + warp * S::kArea;
+  const uint32_t ring = smem_u32(area);
+  const int blocks = (w.count + kBlock - 1) / kBlock;
+  const int mine = blocks > warp ? (blocks - warp + kWarps - 1) / kWarps : 0;   // blocks warp, warp + 4, ...
+
+  // position of key `lane` (< 16) of this warp's i-th block; -1 past the keys or outside the pools
+  auto entry_of = [&](int i) {
+    const int key = w.key0 + (warp + i * kWarps) * kBlock + (lane & 15);
+    return i < mine ? table[min(key, w.keys - 1) >> p.page_shift] : 0;
+  };
+  auto position = [&](int i, int entry) {
+    const int key = w.key0 + (warp + i * kWarps) * kBlock + (lane & 15);
+    const int64_t at = int64_t(entry) * page + (key & (page - 1));
+    const bool inside = at >= 0 && at < p.pool_tokens;
+    if (i < mine && key < w.keys && !inside) set_status(p.status, TA_ERR_BOUNDS);
+    return i < mine && key < w.keys && inside ? int(at) : -1;
+  };
+  constexpr int LPR = D / 8, RPI = 32 / LPR;     // lanes of a row, rows of an instruction
+  const int c = lane % LPR, r = lane / LPR;
+  auto load = [&](int i, int pos) {              // the i-th block into its slot, if there is one
+    if (i < mine) {
+      const uint32_t dst = ring + uint32_t(i % kStages) * (2 * S::kTile);
+      int at[kBlock / RPI];
+#pragma unroll
+      for (int k = 0; k < kBlock / RPI; ++k) at[k] = __shfl_sync(0xffffffffu, pos, k * RPI + r);
+#pragma unroll
+      for (int k = 0; k < kBlock / RPI; ++k) {
+        const int64_t src = pool + int64_t(max(at[k], 0)) * D + c * 8;
+        const uint32_t to = dst + place<D>(k * RPI + r, c), size = at[k] >= 0 ? 16u : 0u;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(p.k + src), "r"(size));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + S::kTile), "l"(p.v + src), "r"(size));
+      }
+    }
+    cp_async_commit();
+  };
+
+  // the first blocks are on their way before the queries are read
+  int entry[kStages];
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) entry[i] = entry_of(i);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) load(i, position(i, entry[i]));
+  int next_entry = entry[kStages - 1];           // of block i + kStages - 1
+
+  // this thread's rows of the fragments: g and g + 8
+  const int g = lane >> 2, t4 = lane & 3;
+  int limit[2];                                  // visible keys of the split
+  uint32_t qa[D / 16][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int row = g + 8 * h, local = w.row0 + row;
+    const bool has = row < w.rows;
+    limit[h] = has ? min(w.keys, w.shift + local / G + 1) - w.key0 : 0;
+    const uint16_t* src = p.q + int64_t(w.token0 + (has ? local / G : 0)) * p.q_st +
+                          int64_t(w.head * G + (has ? local % G : 0)) * p.q_sh + 2 * t4;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      qa[k][h] = has ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
+      qa[k][2 + h] = has ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
+    }
+  }
+
+  float o[D / 8][4];
+#pragma unroll
+  for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, z[2] = {0.f, 0.f};
+  const float scale = p.scale_log2;
+
+  for (int i = 0; i < mine; ++i) {
+    cp_async_wait_group<kStages - 2>();          // block i has landed
+    __syncwarp();                                // and block i - 1, whose slot is filled next, is read
+    const int pos = position(i + kStages - 1, next_entry);
+    next_entry = entry_of(i + kStages);
+    load(i + kStages - 1, pos);
+    const uint32_t kt = ring + uint32_t(i % kStages) * (2 * S::kTile), vt = kt + S::kTile;
+
+    float s[2][4];                               // keys 0-7 and 8-15
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      uint32_t b[4];                             // (keys 0-7 | 8-15) x (dims 0-7 | 8-15) of the step
+      ldm4(b, kt + place<D>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+      mma16816<T>(s[0], qa[k], b[0], b[1]);
+      mma16816<T>(s[1], qa[k], b[2], b[3]);
+    }
+    const int first = (warp + i * kWarps) * kBlock;          // key of the split
+    bool grow = false;
+    float alpha[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float& x = s[n][2 * h + e];
+          x = first + n * 8 + 2 * t4 + e < limit[h] ? x * scale : -INFINITY;
+          top = fmaxf(top, x);
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const bool up = top > m[h] + kRescaleThreshold;        // from -inf: any visible key
+      alpha[h] = up ? fast_exp2(m[h] - top) : 1.f;
+      m[h] = up ? top : m[h];
+      grow |= up;
+      const float m_use = m[h] == -INFINITY ? 0.f : m[h];
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float& x = s[n][2 * h + e];
+          x = fast_exp2(x - m_use);
+          sum += x;
+        }
+      z[h] = z[h] * alpha[h] + sum;
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] *= alpha[e >> 1];
+    }
+    const uint32_t pa[4] = {Elem<T>::pack2(s[0][0], s[0][1]), Elem<T>::pack2(s[0][2], s[0][3]),
+                            Elem<T>::pack2(s[1][0], s[1][1]), Elem<T>::pack2(s[1][2], s[1][3])};
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) {
+      uint32_t b[4];                             // (keys 0-7, 8-15) of dims 0-7, then of dims 8-15
+      ldm4t(b, vt + place<D>((lane & 7) + (((lane >> 3) & 1) << 3), 2 * n + (lane >> 4)));
+      mma16816<T>(o[2 * n], pa, b[0], b[1]);
+      mma16816<T>(o[2 * n + 1], pa, b[2], b[3]);
+    }
+  }
+  cp_async_wait_all();
+
+  // join the warps
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    z[h] += __shfl_xor_sync(0xffffffffu, z[h], 1);
+    z[h] += __shfl_xor_sync(0xffffffffu, z[h], 2);
+    if (t4 == 0) s_m[warp][g + 8 * h] = m[h], s_z[warp][g + 8 * h] = z[h];
+  }
+  __syncwarp();
+  float* mine_o = reinterpret_cast<float*>(area);              // [16][D]: this warp's ring is no longer read
+#pragma unroll
+  for (int n = 0; n < D / 8; ++n) {
+    *reinterpret_cast<float2*>(mine_o + g * D + n * 8 + 2 * t4) = make_float2(o[n][0], o[n][1]);
+    *reinterpret_cast<float2*>(mine_o + (g + 8) * D + n * 8 + 2 * t4) = make_float2(o[n][2], o[n][3]);
+  }
+  __syncthreads();
+  for (int i = tid; i < w.rows * (D / 4); i += kThreads) {
+    const int row = i / (D / 4), col = (i % (D / 4)) * 4;
+    float top = s_m[0][row];
+#pragma unroll
+    for (int k = 1; k < kWarps; ++k) top = fmaxf(top, s_m[k][row]);
+    const float top_use = top == -INFINITY ? 0.f : top;
+    float total = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+      const float weight = fast_exp2(s_m[k][row] - top_use);   // 0 for a warp without keys
+      total += s_z[k][row] * weight;
+      const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(smem + k * S::kArea) + row * D + col);
+      y[0] += x.x * weight, y[1] += x.y * weight, y[2] += x.z * weight, y[3] += x.w * weight;
+    }
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+    const int local = w.row0 + row;
+    const int64_t index = int64_t(w.token0 + local / G) * p.hq + w.head * G + local % G;
+    if (p.splits > 1) {
+      *reinterpret_cast<float4*>(p.part + (int64_t(split) * p.num_tokens * p.hq + index) * D + col) =
+          make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+    } else {
+      *reinterpret_cast<uint2*>(p.out + index * D + col) =
+          make_uint2(Elem<T>::pack2(y[0] * inv, y[1] * inv), Elem<T>::pack2(y[2] * inv, y[3] * inv));
+    }
+    if (col == 0) {
+      const float lse = total > 0.f ? (top + fast_log2(total)) * kLn2 : -INFINITY;
+      if (p.splits > 1)
+        p.part_lse[int64_t(split) * p.num_tokens * p.hq + index] = lse;
+      else if (p.lse)
+        p.lse[index] = lse;
+    }
+  }
+}
+
+template <typename T, int D>
+cudaError_t launch_typed(const ChunkParams& p, int64_t tiles, cudaStream_t stream) {
+  auto kernel = chunk_rows_kernel<T, D>;
+  static std::atomic<uint64_t> configured{0};                // one bit a device
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev >= 64 || !(configured.load() >> dev & 1)) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsSmem<D>::bytes);
+    if (err != cudaSuccess) return err;
+    if (dev < 64) configured.fetch_or(uint64_t(1) << dev);
+  }
+  kernel<<<dim3(unsigned(tiles * p.hk), unsigned(p.splits)), kThreads, RowsSmem<D>::bytes, stream>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_dim(const ChunkParams& p, int64_t tiles, int head_dim, cudaStream_t stream) {
+  if (head_dim == 128) return launch_typed<T, 128>(p, tiles, stream);
+  if (head_dim == 64) return launch_typed<T, 64>(p, tiles, stream);
+  return launch_typed<T, 32>(p, tiles, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_chunk_rows(const ChunkParams& p, int64_t tiles, int head_dim, int dtype, cudaStream_t stream) {
+  return dtype == TA_DTYPE_BF16 ? launch_dim<__nv_bfloat16>(p, tiles, head_dim, stream)
+                                : launch_dim<__half>(p, tiles, head_dim, stream);
+}
+
+}  // namespace ta
