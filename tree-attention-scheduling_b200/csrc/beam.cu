@@ -6,21 +6,21 @@
 // and a request keeps the k best of its beams x vocabulary, sorted, ties to the
 // lowest w * V + t.  Two kernels, the logits read once:
 //
-//  1. beam_slice_kernel, one CTA per (beam row, slice of 8192 tokens).  The
-//     slice stays in registers (32 values a thread).  Within a beam candidates
-//     order by x alone, so the slice's k best by (x, lowest t) are all that can
-//     matter; they are written with the slice's maximum and sum of exponentials.
-//     The k best are found through a bound: if each of the 8 warps gives its
-//     ceil(k/8)-th largest thread maximum, the least of these has at least k
-//     values at or above it, and (on anything but adversarial data) not many
-//     more; those are collected and ranked by counting.  Where more than
-//     kMaxCand values pass (ties, most tokens at -inf), the exact k-th largest
-//     thread maximum under the total order (x, -t) is the bound instead, which
-//     passes at most k threads' values.
+//  1. beam_slice_kernel, one CTA per (beam row, slice of at most 8192 tokens).
+//     The slice stays in registers (32 values a thread).  Within a beam
+//     candidates order by x alone, so the slice's k best by (x, lowest t) are
+//     all that can matter; they are written with the slice's maximum and sum of
+//     exponentials.  The k best are found through a bound: if each of the 8
+//     warps gives its ceil(k/8)-th largest thread maximum, the least of these
+//     has at least k values at or above it, and (on anything but adversarial
+//     data) not many more; those are collected and ranked by counting.  Where
+//     more than kMaxCand values pass (ties, most tokens at -inf), the exact
+//     k-th largest thread maximum under the total order (x, -t) is the bound
+//     instead, which passes at most k threads' values.
 //  2. beam_merge_kernel, one CTA per request: each beam's logsumexp from its
 //     slices in f64, every listed candidate's score in f64 (beams a rounding
-//     apart in f32 would swap), the k-th best list head as the bound, then
-//     ranking by counting.
+//     apart in f32 would swap), a bound from the sorted lists, then ranking by
+//     counting.
 //
 // Bound: HBM for the logits (one read); small batches by the two launches'
 // latency.  MUFU: one ex2 per logit, 16 a clock and SM, 0.7 of the time the
@@ -29,6 +29,7 @@
 
 #include "ta_common.cuh"
 #include "ta_kernels.cuh"
+#include "tc_common.cuh"
 
 namespace ta {
 
@@ -37,9 +38,11 @@ namespace {
 constexpr int kBeamThreads = 256;
 constexpr int kBeamWarps = kBeamThreads / 32;
 constexpr int kPerThread = 32;                              // logits a thread holds
-constexpr int kSlice = kBeamThreads * kPerThread;           // logits of a slice
+constexpr int kSlice = kBeamThreads * kPerThread;           // most logits of a slice
 constexpr int kMaxK = 32;
-constexpr int kMaxCand = kMaxK * kPerThread;                // 1024: what the exact bound can pass
+constexpr float kMaxLogit = 131072.f;                       // larger logits count as this
+constexpr float kLog2eLo = 1.9259629911e-8f;               // log2(e) - kLog2e
+constexpr int kMaxCand = kMaxK * kPerThread;                // 1024: what the exact bounds can pass
 
 struct BeamEntry {     // a listed candidate of a slice
   float x;
@@ -62,7 +65,7 @@ struct BeamParams {
   float* out_scores;              // [R, k]
   int64_t *out_parents, *out_tokens;
   int64_t row_stride;             // elements between beam rows
-  int32_t beams, vocab, k, slices, end_token;
+  int32_t beams, vocab, k, slices, slice, end_token;  // slice: logits of each, a multiple of 32
 };
 
 template <int DT> struct Logit;
@@ -115,23 +118,38 @@ __device__ __forceinline__ uint4 shift_bytes(const uint4& a, const uint4& b, int
                     __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
 }
 
-// Total order of a slice's candidates: larger x first, then the lower token
-// (0: no candidate; -inf maps above it, and -0 equals +0).
-__device__ __forceinline__ uint64_t order_key(float x, int32_t token) {
+// f32 as an unsigned integer of the same order (-0 as +0; 0 is below -inf), and back
+__device__ __forceinline__ uint32_t float_key(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
-  const uint32_t o = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
-  return (uint64_t(o) << 32) | uint32_t(~token);
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float key_float(uint32_t o) {
+  return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-__device__ __forceinline__ int block_count(int v, int* s_warp, int warp, int lane) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  if (lane == 0) s_warp[warp] = v;
-  __syncthreads();
-  int total = 0;
-#pragma unroll
-  for (int i = 0; i < kBeamWarps; ++i) total += s_warp[i];
-  __syncthreads();
-  return total;
+// Total order of a slice's candidates: larger x first, then the lower token (0: no candidate).
+__device__ __forceinline__ uint64_t order_key(float x, int32_t token) {
+  return (uint64_t(float_key(x)) << 32) | uint32_t(~token);
+}
+
+// Rank (how many of the n are before) of every candidate by counting, for the
+// whole CTA: `before(j, i)` compares two, `use(i, rank)` takes the result.  Up
+// to 128 candidates have two or four neighbouring lanes each.
+template <typename Before, typename Use>
+__device__ __forceinline__ void rank_all(int n, const Before& before, const Use& use) {
+  const int parts = n <= kBeamThreads / 4 ? 4 : n <= kBeamThreads / 2 ? 2 : 1;
+  const int per = kBeamThreads / parts, part = threadIdx.x % parts;
+  for (int i0 = 0; i0 < n; i0 += per) {
+    const int i = i0 + threadIdx.x / parts;
+    int rank = 0;
+    if (i < n) {
+#pragma unroll 4
+      for (int j = part; j < n; j += parts) rank += before(j, i);
+    }
+    if (parts > 1) rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    if (parts > 2) rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    if (i < n && part == 0) use(i, rank);
+  }
 }
 
 template <int DT>
@@ -140,11 +158,9 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamParams 
   constexpr int VEC = L::kVec, NV = kPerThread / VEC;
   __shared__ uint64_t s_cand[kMaxCand];
   __shared__ uint64_t s_best[kBeamThreads];
-  __shared__ float s_warp_max[kBeamWarps];
-  __shared__ float s_warp_bound[kBeamWarps];
-  __shared__ double s_warp_sum[kBeamWarps];
+  __shared__ uint32_t s_warp_max[kBeamWarps], s_warp_bound[kBeamWarps];
+  __shared__ float s_warp_sum[kBeamWarps];
   __shared__ int s_count;
-  __shared__ int s_warp_n[kBeamWarps];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int slice = blockIdx.y, k = p.k;
@@ -163,112 +179,124 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamParams 
   const Scalar* base = static_cast<const Scalar*>(p.logits) + row * p.row_stride;
   const int skew = int(reinterpret_cast<uintptr_t>(base) & 15u);
   const int back = skew / int(sizeof(Scalar));               // elements of a vector before its lane's tokens
-  const int64_t first = int64_t(slice) * kSlice;
-  const float score = p.scores[row];
+  const int first = slice * p.slice, end = min(first + p.slice, p.vocab);   // its tokens
   const bool done = p.finished && p.finished[row];
-  const bool dead = !(score > -INFINITY);                  // -inf (or NaN): every candidate is at -inf
-  const bool read = !done && !dead;
-
-  auto token_of = [&](int v, int i) { return int32_t(first + (int64_t(v) * kBeamThreads + tid) * VEC + i); };
-  float x[kPerThread];
+  auto token_of = [&](int v, int i) { return first + (v * kBeamThreads + tid) * VEC + i; };
   uint4 raw[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const int64_t t0 = first + (int64_t(v) * kBeamThreads + tid) * VEC - back;     // tokens of the aligned vector
+    const int t0 = token_of(v, 0) - back;                    // tokens of the aligned vector
     raw[v] = make_uint4(0, 0, 0, 0);
-    if (read && t0 >= 0 && t0 + VEC <= p.vocab) raw[v] = *reinterpret_cast<const uint4*>(base + t0);
+    if (!done && t0 >= 0 && t0 < end && t0 + VEC <= p.vocab) raw[v] = *reinterpret_cast<const uint4*>(base + t0);
   }
+  const bool dead = !(p.scores[row] > -INFINITY);            // -inf (or NaN): every candidate is at -inf
+  if (done || dead) {
+    // Logits do not count.  A finished beam offers its end token alone, at its
+    // unchanged score; whatever else is -inf, where the lowest tokens come first.
+    const bool ends = done && !dead && p.end_token >= first && p.end_token < end;
+    if (tid == 0) p.work.sum[out] = ends ? 1. : 0., p.work.top[out] = ends ? 0.f : -INFINITY;
+    for (int i = tid; i < k; i += kBeamThreads) {
+      int t = first + i - (ends ? 1 : 0);
+      if (ends) t += t >= p.end_token;                       // it comes first
+      entries[i] = ends && i == 0 ? BeamEntry{0.f, p.end_token} : BeamEntry{-INFINITY, t < end ? t : -1};
+    }
+    return;
+  }
+  float x[kPerThread];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    const int64_t t0 = first + (int64_t(v) * kBeamThreads + tid) * VEC;
+    const int t0 = token_of(v, 0);
     if (back) {
       const uint4 a = raw[v];
       uint4 b = make_uint4(__shfl_down_sync(0xffffffffu, a.x, 1), __shfl_down_sync(0xffffffffu, a.y, 1),
                            __shfl_down_sync(0xffffffffu, a.z, 1), __shfl_down_sync(0xffffffffu, a.w, 1));
-      const int64_t t1 = t0 - back + VEC;                   // the next warp's first vector: mostly in L1 by now
-      if (lane == 31) b = read && t1 + VEC <= p.vocab ? *reinterpret_cast<const uint4*>(base + t1) : a;
+      const int t1 = t0 - back + VEC;                        // the next vector: the next lane's
+      if (lane == 31 || t1 >= end) b = t1 + VEC <= p.vocab ? *reinterpret_cast<const uint4*>(base + t1) : a;
       raw[v] = shift_bytes(a, b, skew);
     }
-    // both vectors whole within the row
-    const bool whole = read && t0 - back >= 0 && t0 - back + (back ? 2 : 1) * VEC <= p.vocab;
+    // all of the thread's tokens in the slice (whole multiples of 32 but for the
+    // last), both vectors within the row
+    const bool whole = t0 + VEC <= end && t0 - back >= 0 && t0 - back + (back ? 2 : 1) * VEC <= p.vocab;
     if (whole) {
       L::unpack(raw[v], x + v * VEC);
     } else {
-      // the row's ends, or a beam whose logits do not count: a finished beam
-      // offers its end token alone, with its score unchanged
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int64_t t = t0 + i;
-        float y = -INFINITY;
-        if (t < p.vocab) {
-          if (read)
-            y = L::one(base[t]);
-          else if (done && !dead && t == p.end_token)
-            y = 0.f;
-        }
-        x[v * VEC + i] = y;
-      }
+      for (int i = 0; i < VEC; ++i) x[v * VEC + i] = t0 + i < end ? L::one(base[t0 + i]) : -INFINITY;
     }
   }
   float mine = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) mine = fmaxf(mine, x[i]);     // fmaxf passes over NaN
   // the warp's ceil(k / 8)-th largest thread maximum, ties counted one by one
-  float bound = warp_max(mine), left = mine;
-  if (lane == 0) s_warp_max[warp] = bound;
+  uint32_t left = float_key(mine), warp_bound = __reduce_max_sync(0xffffffffu, left);
+  if (lane == 0) s_warp_max[warp] = warp_bound;
   for (int j = 1; j * kBeamWarps < k; ++j) {
-    const unsigned holders = __ballot_sync(0xffffffffu, left == bound);
-    if (lane == __ffs(holders) - 1) left = -INFINITY;
-    bound = warp_max(left);
+    const unsigned holders = __ballot_sync(0xffffffffu, left == warp_bound);
+    if (lane == __ffs(holders) - 1) left = 0;
+    warp_bound = __reduce_max_sync(0xffffffffu, left);
   }
-  if (lane == 0) s_warp_bound[warp] = bound;
+  if (lane == 0) s_warp_bound[warp] = warp_bound;
   __syncthreads();
-  float m = s_warp_max[0];
-  bound = s_warp_bound[0];
+  uint32_t top_key = s_warp_max[0], bound_key = s_warp_bound[0];
 #pragma unroll
-  for (int i = 1; i < kBeamWarps; ++i) m = fmaxf(m, s_warp_max[i]), bound = fminf(bound, s_warp_bound[i]);
+  for (int i = 1; i < kBeamWarps; ++i) top_key = max(top_key, s_warp_max[i]), bound_key = min(bound_key, s_warp_bound[i]);
+  const float top = key_float(top_key);
+  float bound = bound_key ? key_float(bound_key) : -INFINITY;
 
-  // sum of exp(x - m): f32 over a thread's 32 values, f64 beyond.  An argument
-  // of ex2 below 16 in magnitude is off by 2^-21 at most, at random, so the sum
-  // over many terms keeps about 1e-8.
+  // Sum of 2^(x log2(e) - M) with M = ceil(top log2(e)): whole powers of two
+  // between slices, so they are joined without another exponential.  log2(e) in
+  // two f32 parts keeps an argument t to 2^-24 |t|; with ex2 (2^-22, at random
+  // over the terms) a sum over many terms keeps about 1e-8.  f32 within a warp.
+  float M = ceilf(fminf(top, kMaxLogit) * kLog2e);
+  auto weight = [&](F2 x) {
+    const F2 t = ffma2(x, splat(kLog2eLo), ffma2(x, splat(kLog2e), splat(-M)));
+    F2 e;
+    e.f = make_float2(fast_exp2(t.f.x), fast_exp2(t.f.y));
+    return e;
+  };
   float part = 0.f;
-  if (m > -INFINITY) {
+  if (top > -INFINITY) {
+    F2 two = splat(0.f);
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) part += fast_exp2((x[i] - m) * kLog2e);
+    for (int i = 0; i < kPerThread; i += 2) {
+      F2 d;
+      d.f = make_float2(x[i], x[i + 1]);
+      two = fadd2(two, weight(d));
+    }
+    part = two.f.x + two.f.y;
   }
-  // NaN counts as -inf and +inf as the largest finite value; both are rare
+  // NaN counts as -inf and what is above kMaxLogit as that; both are rare
   // enough to be found by what they do to the sum and the maximum
-  const bool odd = __syncthreads_or(!(part < INFINITY) || m == INFINITY) != 0;
-  if (odd) {
-    m = fminf(m, 3.402823466e38f);
+  if (__syncthreads_or(!(part < INFINITY) || top > kMaxLogit)) {
     part = 0.f;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-      x[i] = fminf(fmaxf(x[i], -INFINITY), 3.402823466e38f);
-      part += m > -INFINITY ? fast_exp2((x[i] - m) * kLog2e) : 0.f;
+      x[i] = fminf(fmaxf(x[i], -INFINITY), kMaxLogit);
+      if (x[i] > -INFINITY) part += weight(splat(x[i])).f.x;
     }
     bound = -INFINITY;                                     // the exact bound below
   }
-  double sum = part;
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-  if (lane == 0) s_warp_sum[warp] = sum;
+  part = warp_sum(part);
+  if (lane == 0) s_warp_sum[warp] = part;
 
-  // candidates at or above the bound
-  int n = 0;
+  // candidates at or above the bound, in any order: ranked below
   if (bound > -INFINITY) {
+    uint32_t hits = 0;
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) n += x[i] >= bound;
-    n = block_count(n, s_warp_n, warp, lane);
-  } else {
-    n = kMaxCand + 1;
-    __syncthreads();
+    for (int i = 0; i < kPerThread; ++i) hits |= x[i] >= bound ? 1u << i : 0u;
+    int at = hits ? atomicAdd(&s_count, __popc(hits)) : 0;
+    for (; hits; hits &= hits - 1, ++at) {                   // few: read again rather than picked from registers
+      const int i = __ffs(hits) - 1, t = token_of(i / VEC, i % VEC);
+      if (at < kMaxCand) s_cand[at] = order_key(L::one(base[t]), t);
+    }
   }
-  if (tid == 0) {
-    double total = 0;
-    for (int i = 0; i < kBeamWarps; ++i) total += s_warp_sum[i];
-    p.work.sum[out] = total;
-    p.work.top[out] = m;
+  __syncthreads();
+  int n = bound > -INFINITY ? s_count : kMaxCand + 1;
+  if (tid < kBeamWarps) {
+    double total = s_warp_sum[tid];
+#pragma unroll
+    for (int off = kBeamWarps / 2; off >= 1; off >>= 1) total += __shfl_xor_sync((1u << kBeamWarps) - 1, total, off);
+    if (tid == 0) p.work.sum[out] = total, p.work.top[out] = top > -INFINITY ? M : -INFINITY;
   }
   uint64_t key_bound = 1;
   if (n > kMaxCand) {
@@ -277,7 +305,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamParams 
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
       const int t = token_of(i / VEC, i % VEC);
-      if (t < p.vocab) best = max(best, order_key(fmaxf(x[i], -INFINITY), t));
+      if (t < end) best = max(best, order_key(fmaxf(x[i], -INFINITY), t));
     }
     s_best[tid] = best;
     __syncthreads();
@@ -285,7 +313,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamParams 
     for (int i = 0; i < kBeamThreads; ++i) above += s_best[i] > best;
     // keys are distinct except 0: at most one thread has exactly k - 1 above it
     __shared__ uint64_t s_bound;
-    if (tid == 0) s_bound = 1;
+    if (tid == 0) s_bound = 1, s_count = 0;
     __syncthreads();
     if (best && above == k - 1) s_bound = best;
     __syncthreads();
@@ -293,7 +321,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamParams 
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
       const int t = token_of(i / VEC, i % VEC);
-      if (t < p.vocab) {
+      if (t < end) {
         const uint64_t key = order_key(fmaxf(x[i], -INFINITY), t);
         if (key >= key_bound) {
           const int at = atomicAdd(&s_count, 1);           // any order: ranked below
@@ -301,116 +329,198 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamParams 
         }
       }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i)
-      if (x[i] >= bound) s_cand[atomicAdd(&s_count, 1)] = order_key(x[i], token_of(i / VEC, i % VEC));
+    __syncthreads();
   }
-  __syncthreads();
   n = min(s_count, kMaxCand);
-  for (int i = tid; i < n; i += kBeamThreads) {
-    const uint64_t key = s_cand[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += s_cand[j] > key;
-    if (rank < k) {
-      const uint32_t o = uint32_t(key >> 32);
-      entries[rank] = {__uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu)), int32_t(~uint32_t(key))};
-    }
-  }
+  rank_all(
+      n, [&](int j, int i) { return s_cand[j] > s_cand[i]; },
+      [&](int i, int rank) {
+        const uint64_t key = s_cand[i];
+        if (rank < k) entries[rank] = {key_float(uint32_t(key >> 32)), int32_t(~uint32_t(key))};
+      });
   for (int i = n + tid; i < k; i += kBeamThreads) entries[i] = {-INFINITY, -1};
 }
 
-struct BeamCand {
-  double score;
-  int64_t flat;      // beam * vocab + token
+struct alignas(16) BeamCand {
+  int64_t key;       // the score in an order-preserving integer form
+  int64_t place;     // beam << 32 | token: the order of ties
 };
 
+// f64 as a signed integer of the same order (-0 as +0), and back
+__device__ __forceinline__ int64_t score_key(double x) {
+  const int64_t b = __double_as_longlong(x + 0.);
+  return b ^ ((b >> 63) & INT64_MAX);
+}
+__device__ __forceinline__ double key_score(int64_t k) { return __longlong_as_double(k ^ ((k >> 63) & INT64_MAX)); }
+// (without short cuts: a branch per comparison costs more than the comparisons)
 __device__ __forceinline__ bool better(const BeamCand& a, const BeamCand& b) {
-  return a.score > b.score || (a.score == b.score && a.flat < b.flat);
+  return (a.key > b.key) | ((a.key == b.key) & (a.place < b.place));
 }
 
+// 2^d for a whole d <= 0 (0 below the range, and for -inf or NaN: an empty slice)
+__device__ __forceinline__ double power_of_two(float d) {
+  return d > -1000.f ? __hiloint2double((1023 + int(d)) << 20, 0) : 0.;
+}
+
+constexpr int kDepths = 4;
+
 __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamParams p) {
-  extern __shared__ __align__(16) unsigned char s_raw[];
-  const int lists = p.beams * p.slices, k = p.k;
-  BeamCand* s_head = reinterpret_cast<BeamCand*>(s_raw);                    // [lists]
-  BeamCand* s_cand = s_head + lists;                                        // [k * k]
-  double* s_score = reinterpret_cast<double*>(s_cand + k * k);              // [beams] score - log(sum)
-  float* s_top = reinterpret_cast<float*>(s_score + p.beams);               // [beams]
-  __shared__ BeamCand s_bound;
+  __shared__ BeamCand s_cand[kMaxCand];
+  __shared__ double s_base[kMaxK];                           // per beam: score - logsumexp
+  __shared__ uint32_t s_warp[kDepths][kBeamWarps], s_bound[kDepths];
+  __shared__ BeamCand s_exact;
   __shared__ int s_count;
 
+  const int lists = p.beams * p.slices, k = p.k;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t request = blockIdx.x;
   const int64_t list0 = request * lists;
-  if (tid == 0) {
-    s_bound = {-INFINITY, INT64_MAX};                       // passes everything
-    s_count = 0;
+  const BeamEntry* entries = p.work.entries + list0 * k;
+  if (tid == 0) s_count = 0;
+  if (tid < kDepths) s_bound[tid] = 0;
+  // half a warp per beam; the beams' scores are inputs of the call: read before the dependency wait
+  const int half = tid >> 4, sub = lane & 15;
+  float score_of[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int w = half + 2 * kBeamWarps * i;
+    score_of[i] = w < p.beams ? p.scores[request * p.beams + w] : 0.f;
   }
-  float score_of[4];                                        // inputs of the call: before the dependency wait
-  for (int w = warp, i = 0; w < p.beams; w += kBeamWarps, ++i) score_of[i] = p.scores[request * p.beams + w];
   pdl_wait();
-  for (int w = warp, i = 0; w < p.beams; w += kBeamWarps, ++i) {
-    const int64_t at = list0 + int64_t(w) * p.slices;
-    float m = -INFINITY;
-    for (int s = lane; s < p.slices; s += 32) m = fmaxf(m, p.work.top[at + s]);
-    m = warp_max(m);
-    double sum = 0;
-    for (int s = lane; s < p.slices; s += 32) {
-      const float t = p.work.top[at + s];
-      if (t > -INFINITY) sum += p.work.sum[at + s] * exp(double(t) - double(m));
+  // A warp has every eighth list (neighbouring lists, those of a beam, go to
+  // different warps: one beam may hold all the best), a lane an entry of each;
+  // the first kHold lists are on their way beside the sums.
+  constexpr int kHold = 16;
+  const int held = min(kHold, (lists - warp + kBeamWarps - 1) / kBeamWarps);
+  auto entry = [&](int list) { return lane < k ? entries[int64_t(list) * k + lane] : BeamEntry{-INFINITY, -1}; };
+  BeamEntry e[kHold];
+#pragma unroll
+  for (int u = 0; u < kHold; ++u) e[u] = u < held ? entry(warp + u * kBeamWarps) : BeamEntry{-INFINITY, -1};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int w = half + 2 * kBeamWarps * i;
+    if (2 * kBeamWarps * i >= p.beams) break;                // uniform
+    const bool has = w < p.beams;
+    const int64_t at = list0 + int64_t(has ? w : 0) * p.slices;
+    // a slice's sum is in units of 2^M, its M in work.top
+    double sum = 0.;
+    float M = -INFINITY;
+    for (int s0 = 0; s0 < p.slices; s0 += 32) {              // two of the lane's slices at a time
+      const int s = s0 + sub;
+      const bool one = has && s < p.slices, two = has && s + 16 < p.slices;
+      const float t1 = one ? p.work.top[at + s] : -INFINITY, t2 = two ? p.work.top[at + s + 16] : -INFINITY;
+      const double p1 = one ? p.work.sum[at + s] : 0., p2 = two ? p.work.sum[at + s + 16] : 0.;
+      float up = fmaxf(M, fmaxf(t1, t2));
+#pragma unroll
+      for (int off = 8; off >= 1; off >>= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, off));
+      sum = sum * power_of_two(M - up) + p1 * power_of_two(t1 - up) + p2 * power_of_two(t2 - up);
+      M = up;
     }
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (lane == 0) {
-      s_top[w] = m;
-      s_score[w] = m > -INFINITY ? double(score_of[i]) - log(sum) : -INFINITY;
-    }
+    for (int off = 8; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (has && sub == 0)
+      s_base[w] = M > -INFINITY ? double(score_of[i]) - (double(M) + log2(sum)) * 0.69314718055994530942 : -INFINITY;
   }
   __syncthreads();
-  auto candidate = [&](int list, const BeamEntry& e) {
-    const int w = list / p.slices;
-    BeamCand c;
-    c.flat = int64_t(w) * p.vocab + e.token;
-    c.score = e.x > -INFINITY ? (double(e.x) - double(s_top[w])) + s_score[w] : -INFINITY;
-    return c;
+  auto score = [&](int w, float x) { return x > -INFINITY ? double(x) + s_base[w] : -INFINITY; };
+  // The same in f32 (f64 is slow here), less or more a margin for its rounding:
+  // the bound is taken from lower values, candidates pass by their upper ones.
+  auto rough = [&](int w, float x, float side) {
+    const float c = float(s_base[w]);
+    return x > -INFINITY && c > -INFINITY ? x + c + side * 4e-7f * (fabsf(x) + fabsf(c)) : -INFINITY;
   };
-  for (int i = tid; i < lists; i += kBeamThreads) {
-    const BeamEntry e = p.work.entries[(list0 + i) * k];
-    s_head[i] = e.token >= 0 ? candidate(i, e) : BeamCand{-INFINITY, INT64_MAX};
+  // beam of a list (exact: lists stay far below 2^20)
+  const float per_slice = 1.f / float(p.slices);
+  auto beam_of = [&](int list) { return int((float(list) + 0.5f) * per_slice); };
+  // A bound that at least k candidates reach: the lists are sorted, so where r
+  // lists have their d-th entry at or above it there are r d candidates.  With
+  // each warp's best d-th entry, the r-th largest of the 8 warps' is such a
+  // bound for r = ceil(k / d); the best of the depths d = ceil(k / 8), 2 d, 4 d
+  // and 8 d leaves few more than k.  Lane d - 1 sees a warp's d-th entries.
+  const int depth0 = (k + kBeamWarps - 1) / kBeamWarps;
+  float low = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < kHold; ++u)
+    if (e[u].token >= 0) low = fmaxf(low, rough(beam_of(warp + u * kBeamWarps), e[u].x, -1.f));
+  for (int list = warp + kHold * kBeamWarps; list < lists; list += kBeamWarps) {
+    const BeamEntry f = entry(list);
+    if (f.token >= 0) low = fmaxf(low, rough(beam_of(list), f.x, -1.f));
   }
+#pragma unroll
+  for (int u = 0; u < kDepths; ++u)
+    if (lane == (depth0 << u) - 1) s_warp[u][warp] = float_key(low);
   __syncthreads();
-  // the k-th best head: at least k candidates are as good, in at most k lists
-  for (int i = tid; i < lists; i += kBeamThreads) {
-    const BeamCand c = s_head[i];
-    int above = 0;
-    for (int j = 0; j < lists; ++j) above += better(s_head[j], c);
-    if (above == k - 1 && c.flat != INT64_MAX) s_bound = c;
-  }
-  __syncthreads();
-  const BeamCand bound = s_bound;
-  const int total = lists * k;
-  for (int i = tid; i < total; i += kBeamThreads) {
-    const BeamEntry e = p.work.entries[list0 * k + i];
-    if (e.token < 0) continue;
-    const BeamCand c = candidate(i / k, e);
-    if (!better(bound, c)) {
-      const int at = atomicAdd(&s_count, 1);                // any order: ranked below
-      if (at < k * k) s_cand[at] = c;
-    }
-  }
-  __syncthreads();
-  const int n = min(s_count, k * k);
-  for (int i = tid; i < n; i += kBeamThreads) {
-    const BeamCand c = s_cand[i];
+  if (tid < kDepths * kBeamWarps) {
+    const int u = tid / kBeamWarps, i = tid % kBeamWarps, d = depth0 << u;   // (d may pass 32: then nothing is kept)
+    const uint32_t mine = s_warp[u][i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += better(s_cand[j], c);
-    if (rank < k) {
-      const int64_t o = request * k + rank;
-      p.out_scores[o] = float(c.score);
-      p.out_parents[o] = c.flat / p.vocab;
-      p.out_tokens[o] = c.flat % p.vocab;
-    }
+#pragma unroll
+    for (int j = 0; j < kBeamWarps; ++j) rank += (s_warp[u][j] > mine) | ((s_warp[u][j] == mine) & (j < i));
+    if (d <= k && rank == (k + d - 1) / d - 1) s_bound[u] = mine;
   }
+  __syncthreads();
+  uint32_t bound = s_bound[0];
+#pragma unroll
+  for (int u = 1; u < kDepths; ++u) bound = max(bound, s_bound[u]);
+
+  auto collect = [&](int list, const BeamEntry& f) {
+    const int w = beam_of(list);
+    if (f.token >= 0 && float_key(rough(w, f.x, 1.f)) >= bound) {
+      const int at = atomicAdd(&s_count, 1);                 // any order: ranked below
+      if (at < kMaxCand) s_cand[at] = {score_key(score(w, f.x)), (int64_t(w) << 32) | f.token};
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < kHold; ++u)
+    if (u < held) collect(warp + u * kBeamWarps, e[u]);
+  for (int list = warp + kHold * kBeamWarps; list < lists; list += kBeamWarps) collect(list, entry(list));
+  __syncthreads();
+  int n = s_count;
+  if (n > kMaxCand) {
+    // Equal scores throughout.  The k-th best head in the exact order passes at
+    // most k entries of k lists (all entries where there are fewer lists).
+    auto exact = [&](int list, const BeamEntry& e) {
+      const int w = list / p.slices;
+      return BeamCand{score_key(score(w, e.x)), (int64_t(w) << 32) | e.token};
+    };
+    if (tid == 0) s_count = 0, s_exact = {INT64_MIN, INT64_MAX};
+    __syncthreads();
+    for (int i = tid; i < lists; i += kBeamThreads) {
+      const BeamEntry e = entries[int64_t(i) * k];
+      if (e.token < 0) continue;
+      const BeamCand c = exact(i, e);
+      int above = 0;
+      for (int j = 0; j < lists; ++j) {
+        const BeamEntry f = entries[int64_t(j) * k];
+        above += f.token >= 0 && better(exact(j, f), c);
+      }
+      if (above == k - 1) s_exact = c;
+    }
+    __syncthreads();
+    const BeamCand least = s_exact;
+    for (int i = tid; i < lists * k; i += kBeamThreads) {
+      const BeamEntry e = entries[i];
+      if (e.token < 0) continue;
+      const BeamCand c = exact(i / k, e);
+      if (!better(least, c)) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kMaxCand) s_cand[at] = c;
+      }
+    }
+    __syncthreads();
+    n = min(s_count, kMaxCand);
+  }
+  rank_all(
+      n, [&](int j, int i) { return better(s_cand[j], s_cand[i]); },
+      [&](int i, int rank) {
+        const BeamCand c = s_cand[i];
+        if (rank < k) {
+          const int64_t o = request * k + rank;
+          p.out_scores[o] = float(key_score(c.key));
+          p.out_parents[o] = c.place >> 32;
+          p.out_tokens[o] = c.place & 0xffffffff;
+        }
+      });
 }
 
 // ---- reordering ---------------------------------------------------------------
@@ -491,9 +601,7 @@ extern "C" int ta_beam_select(const void* logits, int64_t row_stride, const floa
   const int slices = beam_slices(vocab);
   const int64_t rows = int64_t(num_requests) * num_beams;
   if (rows > INT32_MAX) return TA_ERR_UNSUPPORTED;
-  const size_t smem = size_t(num_beams) * slices * sizeof(BeamCand) + size_t(k) * k * sizeof(BeamCand) +
-                      size_t(num_beams) * (sizeof(double) + sizeof(float));
-  if (smem > 48 * 1024) return TA_ERR_UNSUPPORTED;
+  if (slices > 65535) return TA_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(logits) % size) || (reinterpret_cast<uintptr_t>(workspace) & 15u)) return TA_ERR_ARG;
   if (workspace_bytes < ta_beam_workspace_bytes(num_requests, num_beams, vocab, k, dtype)) return TA_ERR_TOO_LARGE;
   BeamParams p{};
@@ -502,6 +610,7 @@ extern "C" int ta_beam_select(const void* logits, int64_t row_stride, const floa
   p.finished = finished;
   p.row_stride = row_stride;
   p.beams = num_beams, p.vocab = vocab, p.k = k, p.slices = slices, p.end_token = end_token;
+  p.slice = ((vocab + slices - 1) / slices + 31) / 32 * 32;   // alike, so that every thread has a share
   p.out_scores = out_scores, p.out_parents = out_parents, p.out_tokens = out_tokens;
   const int64_t n = rows * slices;
   p.work.sum = static_cast<double*>(workspace);
@@ -517,7 +626,7 @@ extern "C" int ta_beam_select(const void* logits, int64_t row_stride, const floa
     beam_slice_kernel<TA_DTYPE_F32><<<grid, kBeamThreads, 0, s>>>(p);
   cudaError_t err = cudaGetLastError();
   if (err == cudaSuccess)
-    err = launch_dependent(beam_merge_kernel, dim3(unsigned(num_requests)), dim3(kBeamThreads), smem, s, p);
+    err = launch_dependent(beam_merge_kernel, dim3(unsigned(num_requests)), dim3(kBeamThreads), 0, s, p);
   return err == cudaSuccess ? TA_OK : TA_ERR_LAUNCH;
 }
 

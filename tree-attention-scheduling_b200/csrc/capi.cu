@@ -3,12 +3,35 @@
 // The host side only validates arguments, resolves the plan layout into kernel
 // parameter blocks and launches on the caller's stream: no allocation, no
 // synchronisation, so every call can be captured into a CUDA graph.
+#include <atomic>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
 
 #include "ta_common.cuh"
 #include "ta_kernels.cuh"
+
+namespace ta {
+
+int sm_count() {
+  static std::atomic<int> cached[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return 148;
+  }
+  int sms = cached[dev].load();
+  if (!sms) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) {
+      cudaGetLastError();
+      sms = 148;
+    }
+    cached[dev].store(sms);
+  }
+  return sms;
+}
+
+}  // namespace ta
 
 using namespace ta;
 

@@ -582,28 +582,6 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(ChunkPara
 }
 
 // ---- host ---------------------------------------------------------------------
-struct Split {
-  int splits, tiles;
-};
-
-int sm_count() {
-  static std::atomic<int> cached[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
-    cudaGetLastError();
-    return 148;
-  }
-  int sms = cached[dev].load();
-  if (!sms) {
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) {
-      cudaGetLastError();
-      sms = 148;
-    }
-    cached[dev].store(sms);
-  }
-  return sms;
-}
-
 // Which kernel runs and how the keys are cut, from sizes known on the host.
 struct Plan {
   bool small;          // the small-row kernel

@@ -15,9 +15,12 @@
 // fraction is rounded to f32 (2^-25 turns) for sincospif.  The rotary_dim / 2
 // sines of a token are computed once per CTA and shared by all its heads.
 //
-// Bound: HBM.  A CTA is one token; a thread owns one 16-byte chunk of a row
-// (always the same columns: its cosines stay in registers) and keeps four rows
-// in flight.
+// Bound: HBM, if the instructions stay few: a thread owns the two 16-byte chunks
+// of a row that hold both elements of eight pairs (so no exchange between
+// lanes), always the same columns and rows: its pointers, weights and, for a
+// token, sines and cosines are set up once.  A CTA walks tokens with up to 64
+// rows (head_dim 128); the next token's sines are computed while the current
+// one's rows are under way, one barrier a token.
 #include <algorithm>
 
 #include "ta_common.cuh"
@@ -27,8 +30,12 @@ namespace ta {
 
 namespace {
 
-constexpr int kRotaryThreads = 256;
-constexpr int kRowsInFlight = 4;
+constexpr int kRotaryThreads = 128;
+// Rows of a thread and resident CTAs an SM: three rows for long inputs (16384
+// tokens of 32 + 8 + 8 heads: 78 us; one row 87, four rows 79); one row while
+// the CTAs fit one wave, where it is latency that counts (16 tokens: 2.9 us
+// against 3.8 with three rows).
+template <int R> constexpr int kCtas = R == 1 ? 8 : 5;
 
 struct RotaryParams {
   const uint16_t *q, *k, *v;
@@ -59,14 +66,14 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
   }
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_append_kernel(RotaryParams p) {
-  constexpr int LPR = D / 8;                    // lanes (16-byte chunks) of a row
-  __shared__ float s_cos[D / 2], s_sin[D / 2];
-  const int tid = threadIdx.x, lane = tid & 31;
-  const int64_t token = blockIdx.x;
+template <typename T, int D, bool PAIRS, int R>  // PAIRS: (2i, 2i + 1), else (i, i + rotary_dim / 2); R rows a thread
+__global__ void __launch_bounds__(kRotaryThreads, kCtas<R>) rotary_append_kernel(const __grid_constant__ RotaryParams p) {
+  constexpr int LPR = D / 16;                   // lanes of a row
+  constexpr int RPP = kRotaryThreads / LPR;     // rows of a pass of the CTA
+  __shared__ __align__(16) float s_cos[2][D / 2], s_sin[2][D / 2];
+  const int tid = threadIdx.x;
 
-  if (p.klen && token == 0) {                   // a captured decode step's first layer: the tails' lengths
+  if (p.klen && blockIdx.x == 0 && blockIdx.y == 0) {   // a captured decode step's first layer: the tails' lengths
     const int64_t value = *p.count + p.offset;
     for (int i = tid; i < p.num_tails; i += kRotaryThreads) {
       const int j = p.tail_jobs[i];
@@ -76,106 +83,129 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_append_kernel(RotaryPar
         p.klen[j] = int32_t(value);
     }
   }
-  if (token >= p.num_tokens) return;            // a launch for the tails alone
-
-  const int c = tid % LPR;                      // this thread's chunk of every row it handles
   const int rows = p.hq + 2 * p.hk;
-  const int64_t target = p.targets[token];
-  const bool stored = target >= 0 && target < p.pool_tokens;
-  if (!stored && target != -1 && tid == 0) set_status(p.status, TA_ERR_BOUNDS);
+  int token = blockIdx.x;
+  if (token >= p.num_tokens || rows == 0) return;
 
-  float cosv[8], sinv[8];
-  bool have_angles = false;
-  // lane that holds the other half of this lane's pairs, and the sign of its term
-  const int hl = p.half / 8;
-  const bool turns = 8 * c < 2 * p.half;
-  const bool first = c < hl;
-  const int partner = p.interleaved || !turns ? lane : (first ? lane + hl : lane - hl);
-
-  for (int row0 = tid / LPR; row0 - tid / LPR < rows; row0 += kRowsInFlight * (kRotaryThreads / LPR)) {
-    uint4 raw[kRowsInFlight];
+  // this thread's pairs 8j .. 8j + 7 and the chunks they lie in
+  const int j = tid % LPR, hl = p.half / 8;
+  const bool turns = j < hl;
+  const int c0 = PAIRS ? 2 * j : turns ? j : 2 * j, c1 = PAIRS || !turns ? c0 + 1 : j + hl;
+  // its rows: q heads, then k, then v
+  const uint16_t* src[R];
+  uint16_t* dst[R];
+  int kind[R];                      // 0 q, 1 k, 2 v, 3 none
 #pragma unroll
-    for (int u = 0; u < kRowsInFlight; ++u) {
-      const int row = row0 + u * (kRotaryThreads / LPR);
-      raw[u] = make_uint4(0, 0, 0, 0);
-      if (row < p.hq)
-        raw[u] = *reinterpret_cast<const uint4*>(p.q + token * p.q_st + int64_t(row) * p.q_sh + c * 8);
-      else if (row < p.hq + p.hk)
-        raw[u] = *reinterpret_cast<const uint4*>(p.k + token * p.k_st + int64_t(row - p.hq) * p.k_sh + c * 8);
-      else if (row < rows)
-        raw[u] = *reinterpret_cast<const uint4*>(p.v + token * p.v_st + int64_t(row - p.hq - p.hk) * p.v_sh + c * 8);
+  for (int u = 0; u < R; ++u) {
+    const int row = (blockIdx.y * R + u) * RPP + tid / LPR;
+    if (row < p.hq) {
+      kind[u] = 0;
+      src[u] = p.q + token * p.q_st + int64_t(row) * p.q_sh;
+      dst[u] = p.q_out + int64_t(row) * D;
+    } else if (row < p.hq + p.hk) {
+      kind[u] = 1;
+      src[u] = p.k + token * p.k_st + int64_t(row - p.hq) * p.k_sh;
+      dst[u] = p.kpool + int64_t(row - p.hq) * p.pool_tokens * D;
+    } else if (row < rows) {
+      kind[u] = 2;
+      src[u] = p.v + token * p.v_st + int64_t(row - p.hq - p.hk) * p.v_sh;
+      dst[u] = p.vpool + int64_t(row - p.hq - p.hk) * p.pool_tokens * D;
+    } else {
+      kind[u] = 3;
+      src[u] = nullptr;
+      dst[u] = nullptr;
     }
-    if (!have_angles) {                         // behind the first loads
-      have_angles = true;
-      const double turn = double(p.positions[token]) * 0.15915494309189533577;   // 1 / 2 pi
-      for (int i = tid; i < p.half; i += kRotaryThreads) {
-        const double t = turn * double(p.inv_freq[i]);
-        float s, co;
-        sincospif(2.f * float(t - rint(t)), &s, &co);
-        s_cos[i] = co * p.factor;
-        s_sin[i] = s * p.factor;
-      }
-      __syncthreads();
-      if (turns) {
+  }
+  auto sines = [&](int tok, int buffer) {
+    const double turn = double(p.positions[tok]) * 0.15915494309189533577;       // 1 / 2 pi
+    for (int i = tid; i < p.half; i += kRotaryThreads) {
+      const double t = turn * double(p.inv_freq[i]);
+      float s, co;
+      sincospif(2.f * float(t - rint(t)), &s, &co);
+      s_cos[buffer][i] = co * p.factor;
+      s_sin[buffer][i] = s * p.factor;
+    }
+  };
+
+  const bool norm = p.q_weight || p.k_weight;
+  sines(token, 0);
+  for (int buffer = 0;; buffer ^= 1) {
+    uint4 raw[R][2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int pair = p.interleaved ? 4 * c + i / 2 : 8 * (first ? c : c - hl) + i;
-          cosv[i] = s_cos[pair];
-          // out = own * cos + other * sin', with -sin for the first element of a pair
-          const bool leads = p.interleaved ? (i & 1) == 0 : first;
-          sinv[i] = leads ? -s_sin[pair] : s_sin[pair];
+    for (int u = 0; u < R; ++u) {
+      if (kind[u] == 3) break;                  // rows only end: later ones are none as well
+      raw[u][0] = *reinterpret_cast<const uint4*>(src[u] + c0 * 8);
+      raw[u][1] = *reinterpret_cast<const uint4*>(src[u] + c1 * 8);
+      src[u] += (kind[u] == 0 ? p.q_st : kind[u] == 1 ? p.k_st : p.v_st) * int64_t(gridDim.x);
+    }
+    const int64_t target = p.targets[token];
+    const bool stored = target >= 0 && target < p.pool_tokens;
+    if (!stored && target != -1 && tid == 0) set_status(p.status, TA_ERR_BOUNDS);
+    const int following = token + gridDim.x;
+    __syncthreads();                            // this token's sines are there, the last one's are read
+    float co[8], si[8];
+    if (turns) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        *reinterpret_cast<float4*>(co + i) = *reinterpret_cast<const float4*>(&s_cos[buffer][8 * j + i]);
+        *reinterpret_cast<float4*>(si + i) = *reinterpret_cast<const float4*>(&s_sin[buffer][8 * j + i]);
+      }
+    }
+    if (following < p.num_tokens) sines(following, buffer ^ 1);
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      if (__all_sync(0xffffffffu, kind[u] == 3)) break;
+      uint4 lo = raw[u][0], hi = raw[u][1];
+      if (__any_sync(0xffffffffu, kind[u] < 2)) {
+        float x[16];
+        {
+          float a[8], b[8];
+          unpack8<T>(lo, a);
+          unpack8<T>(hi, b);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = a[i], x[8 + i] = b[i];
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) cosv[i] = 1.f, sinv[i] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kRowsInFlight; ++u) {
-      const int row = row0 + u * (kRotaryThreads / LPR);
-      const bool is_q = row < p.hq, is_k = !is_q && row < p.hq + p.hk;
-      if (!__any_sync(0xffffffffu, row < rows)) break;
-      uint4 result = raw[u];
-      if (__any_sync(0xffffffffu, is_q || is_k)) {
-        float x[8];
-        unpack8<T>(raw[u], x);
-        if (p.q_weight || p.k_weight) {
+        if (norm) {
           float sum = 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
+          for (int i = 0; i < 16; ++i) sum += x[i] * x[i];
 #pragma unroll
           for (int off = LPR / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-          const uint16_t* w = is_q ? p.q_weight : is_k ? p.k_weight : nullptr;
-          if (w) {
+          const uint16_t* weight = kind[u] == 0 ? p.q_weight : kind[u] == 1 ? p.k_weight : nullptr;
+          if (weight) {
             const float scale = rsqrtf(sum * (1.f / D) + p.eps);
-            float wf[8];
-            unpack8<T>(*reinterpret_cast<const uint4*>(w + c * 8), wf);
+            float a[8], b[8];
+            unpack8<T>(*reinterpret_cast<const uint4*>(weight + c0 * 8), a);
+            unpack8<T>(*reinterpret_cast<const uint4*>(weight + c1 * 8), b);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * scale * wf[i];
+            for (int i = 0; i < 8; ++i) x[i] *= scale * a[i], x[8 + i] *= scale * b[i];
           }
         }
-        float y[8];
-        if (p.interleaved) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = x[i] * cosv[i] + (turns ? x[i ^ 1] * sinv[i] : 0.f);
-        } else {
+        if (turns) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float other = __shfl_sync(0xffffffffu, x[i], partner);
-            y[i] = x[i] * cosv[i] + (turns ? other * sinv[i] : 0.f);
+            float& a = x[PAIRS ? 2 * i : i];
+            float& b = x[PAIRS ? 2 * i + 1 : 8 + i];
+            const float ra = a * co[i] - b * si[i];
+            b = b * co[i] + a * si[i];
+            a = ra;
           }
         }
-        if (is_q || is_k)
-          result = make_uint4(Elem<T>::pack2(y[0], y[1]), Elem<T>::pack2(y[2], y[3]), Elem<T>::pack2(y[4], y[5]),
-                              Elem<T>::pack2(y[6], y[7]));
+        if (kind[u] < 2) {
+          lo = make_uint4(Elem<T>::pack2(x[0], x[1]), Elem<T>::pack2(x[2], x[3]), Elem<T>::pack2(x[4], x[5]),
+                          Elem<T>::pack2(x[6], x[7]));
+          hi = make_uint4(Elem<T>::pack2(x[8], x[9]), Elem<T>::pack2(x[10], x[11]), Elem<T>::pack2(x[12], x[13]),
+                          Elem<T>::pack2(x[14], x[15]));
+        }
       }
-      if (is_q)
-        *reinterpret_cast<uint4*>(p.q_out + (token * p.hq + row) * D + c * 8) = result;
-      else if (is_k && stored)
-        *reinterpret_cast<uint4*>(p.kpool + (int64_t(row - p.hq) * p.pool_tokens + target) * D + c * 8) = result;
-      else if (!is_k && row < rows && stored)
-        *reinterpret_cast<uint4*>(p.vpool + (int64_t(row - p.hq - p.hk) * p.pool_tokens + target) * D + c * 8) = result;
+      if (kind[u] == 0 || (kind[u] < 3 && stored)) {
+        uint16_t* out = dst[u] + (kind[u] == 0 ? int64_t(token) * p.hq : target) * D;
+        *reinterpret_cast<uint4*>(out + c0 * 8) = lo;
+        *reinterpret_cast<uint4*>(out + c1 * 8) = hi;
+      }
     }
+    token = following;
+    if (token >= p.num_tokens) break;
   }
 }
 
@@ -183,15 +213,27 @@ bool rows16(const void* p, int64_t st, int64_t sh) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && st >= 0 && sh >= 0 && (st & 7) == 0 && (sh & 7) == 0;
 }
 
-template <typename T>
-void launch_rotary(const RotaryParams& p, int head_dim, cudaStream_t stream) {
-  const unsigned grid = unsigned(std::max(1, p.num_tokens));
-  if (head_dim == 128)
-    rotary_append_kernel<T, 128><<<grid, kRotaryThreads, 0, stream>>>(p);
-  else if (head_dim == 64)
-    rotary_append_kernel<T, 64><<<grid, kRotaryThreads, 0, stream>>>(p);
+template <typename T, int D, int R>
+void launch_rotary(const RotaryParams& p, int sms, cudaStream_t stream) {
+  constexpr int kRows = kRotaryThreads / (D / 16) * R;                 // rows of a CTA
+  const int batches = std::max(1, (p.hq + 2 * p.hk + kRows - 1) / kRows);
+  if (R == 1 && int64_t(p.num_tokens) * batches > int64_t(sms) * kCtas<1>) return launch_rotary<T, D, 3>(p, sms, stream);
+  // enough CTAs to fill the GPU, each with its share of the tokens
+  const dim3 grid(std::max(1, std::min(p.num_tokens, std::max(1, sms * kCtas<R> / batches))), batches);
+  if (p.interleaved)
+    rotary_append_kernel<T, D, true, R><<<grid, kRotaryThreads, 0, stream>>>(p);
   else
-    rotary_append_kernel<T, 32><<<grid, kRotaryThreads, 0, stream>>>(p);
+    rotary_append_kernel<T, D, false, R><<<grid, kRotaryThreads, 0, stream>>>(p);
+}
+
+template <typename T>
+void launch_rotary(const RotaryParams& p, int head_dim, int sms, cudaStream_t stream) {
+  if (head_dim == 128)
+    launch_rotary<T, 128, 1>(p, sms, stream);
+  else if (head_dim == 64)
+    launch_rotary<T, 64, 1>(p, sms, stream);
+  else
+    launch_rotary<T, 32, 1>(p, sms, stream);
 }
 
 }  // namespace
@@ -253,8 +295,8 @@ extern "C" int ta_rotary_append(const void* q, int64_t q_stride_token, int64_t q
   p.num_tails = klen ? num_tails : 0;
   p.offset = offset, p.num_jobs = num_jobs;
   if (dtype == TA_DTYPE_BF16)
-    launch_rotary<__nv_bfloat16>(p, head_dim, static_cast<cudaStream_t>(stream));
+    launch_rotary<__nv_bfloat16>(p, head_dim, sm_count(), static_cast<cudaStream_t>(stream));
   else
-    launch_rotary<__half>(p, head_dim, static_cast<cudaStream_t>(stream));
+    launch_rotary<__half>(p, head_dim, sm_count(), static_cast<cudaStream_t>(stream));
   return cudaGetLastError() == cudaSuccess ? TA_OK : TA_ERR_LAUNCH;
 }
