@@ -1,0 +1,387 @@
+// Python calls of the prompt and beam-search operators: argument checks, output
+// and workspace tensors and the launch, in one step from Python.
+//
+// Going through ctypes a call of these entry points costs 20 to 30 us of host
+// time (30 arguments converted, a dozen tensor properties read, two or three
+// tensors made), several times what a small call takes on the GPU; from here it
+// is about 5.  The kernels stay behind the C ABI: `bind` receives the addresses
+// of the entry points of the library that tree_attention._lib has loaded and
+// checked.  Every function raises ValueError for arguments it does not take and
+// RuntimeError for an error code; no C++ exception leaves it.
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
+
+#include <cmath>
+#include <cstring>
+
+#include "tree_attn.h"
+
+namespace {
+
+// ---- entry points of the kernel library ---------------------------------------
+struct Entry {
+  decltype(&ta_error_string) error_string;
+  decltype(&ta_rotary_append) rotary_append;
+  decltype(&ta_chunk_workspace_bytes) chunk_workspace_bytes;
+  decltype(&ta_chunk_attention) chunk_attention;
+  decltype(&ta_beam_workspace_bytes) beam_workspace_bytes;
+  decltype(&ta_beam_select) beam_select;
+  decltype(&ta_beam_reorder) beam_reorder;
+} entry{};
+
+// ---- arguments ------------------------------------------------------------------
+const at::Tensor& tensor(PyObject* o, const char* what) {
+  TORCH_CHECK_TYPE(THPVariable_Check(o), what, " must be a tensor");
+  return THPVariable_Unpack(o);
+}
+at::Tensor optional(PyObject* o, const char* what) { return o == Py_None ? at::Tensor() : tensor(o, what); }
+int64_t integer(PyObject* o) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+double real(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw python_error();
+  return v != 0;
+}
+int32_t narrow(int64_t v, const char* what) {
+  TORCH_CHECK_VALUE(v >= INT32_MIN && v <= INT32_MAX, what, " does not fit 32 bits");
+  return int32_t(v);
+}
+void count_args(Py_ssize_t got, Py_ssize_t want) { TORCH_CHECK_TYPE(got == want, "expected ", want, " arguments, got ", got); }
+
+// ---- tensors --------------------------------------------------------------------
+int32_t dtype_code(at::ScalarType t) {
+  return t == at::kBFloat16 ? TA_DTYPE_BF16 : t == at::kHalf ? TA_DTYPE_F16 : t == at::kFloat ? TA_DTYPE_F32 : 0;
+}
+bool half_type(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+bool aligned16(const at::Tensor& x) { return (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15u) == 0; }
+void* ptr(const at::Tensor& x) { return x.defined() ? x.data_ptr() : nullptr; }
+at::Tensor packed(const at::Tensor& x) { return x.is_contiguous() ? x : x.contiguous(); }
+
+// x [N, H, D] itself where its rows can be read in 16-byte pieces, else a copy.
+at::Tensor rows16(const at::Tensor& x) {
+  if (x.stride(2) != 1 || (x.stride(0) & 7) || (x.stride(1) & 7) || !aligned16(x))
+    return x.clone(at::MemoryFormat::Contiguous);
+  return x;
+}
+// Whether the memory ranges of two tensors meet.
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  if (!a.numel() || !b.numel()) return false;
+  auto span = [](const at::Tensor& x) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < x.dim(); ++i) last += (x.size(i) - 1) * x.stride(i);
+    const uintptr_t first = reinterpret_cast<uintptr_t>(x.data_ptr());
+    return std::pair<uintptr_t, uintptr_t>(first, first + uintptr_t(last + 1) * x.element_size());
+  };
+  const auto x = span(a), y = span(b);
+  return x.first < y.second && y.first < x.second;
+}
+void one_device(const char* what, const at::Device& device, std::initializer_list<const at::Tensor*> all) {
+  for (const at::Tensor* t : all)
+    TORCH_CHECK_VALUE(!t->defined() || t->device() == device, what, ": all tensors must be CUDA tensors on one device");
+}
+void check_pools(const char* what, const at::Tensor& kp, const at::Tensor& vp) {
+  TORCH_CHECK_VALUE(kp.dim() == 3 && vp.sizes() == kp.sizes() && kp.is_contiguous() && vp.is_contiguous(), what,
+                    " wants contiguous [HK, T, D] pools of one shape");
+  TORCH_CHECK_VALUE(aligned16(kp) && aligned16(vp), what, ": the pools must be 16-byte aligned");
+}
+void check_status(const char* what, const at::Tensor& status, const at::Device& device) {
+  TORCH_CHECK_VALUE(!status.defined() || (status.device() == device && status.scalar_type() == at::kInt && status.numel() >= 1),
+                    what, ": status must be an int32 CUDA tensor on the pools' device");
+}
+void* stream_of(const at::Device& device) { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
+void done(int rc, const char* what) {
+  TORCH_CHECK(rc == TA_OK, what, " failed: ", entry.error_string(rc), " (code ", rc, ")");
+}
+
+bool head_dim_ok(int64_t d) { return d == 32 || d == 64 || d == 128; }
+
+// ---- the operators ----------------------------------------------------------------
+PyObject* rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  count_args(n_args, 20);
+  at::Tensor q = tensor(a[0], "q"), k = tensor(a[1], "k"), v = tensor(a[2], "v");
+  at::Tensor positions = tensor(a[3], "positions"), freq = tensor(a[4], "inv_freq");
+  const at::Tensor &kp = tensor(a[5], "kp"), &vp = tensor(a[6], "vp");
+  at::Tensor targets = tensor(a[7], "targets");
+  const bool interleaved = truth(a[8]);
+  const double factor = real(a[9]);
+  at::Tensor qw = optional(a[10], "q_weight"), kw = optional(a[11], "k_weight");
+  const double eps = real(a[12]);
+  at::Tensor out = optional(a[13], "out");
+  const at::Tensor status = optional(a[14], "status"), klen = optional(a[15], "klen"), tails = optional(a[16], "tails"),
+                   count = optional(a[17], "count");
+  const int32_t offset = narrow(integer(a[18]), "offset"), jobs = narrow(integer(a[19]), "num_jobs");
+
+  TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes() && q.size(0) == k.size(0) &&
+                        q.size(2) == k.size(2),
+                    "rotary_append wants q [N, HQ, D] and k, v [N, HK, D]");
+  const int64_t n = q.size(0), hq = q.size(1), dim = q.size(2), hk = k.size(1);
+  const at::Device device = q.device();
+  TORCH_CHECK_VALUE(q.is_cuda(), "rotary_append: all tensors must be CUDA tensors on one device");
+  one_device("rotary_append", device,
+             {&k, &v, &positions, &freq, &kp, &vp, &targets, &qw, &kw, &out, &klen, &tails, &count});
+  TORCH_CHECK_VALUE(head_dim_ok(dim), "rotary_append: head_dim must be 32, 64 or 128");
+  check_pools("rotary_append", kp, vp);
+  TORCH_CHECK_VALUE(kp.size(0) == hk && kp.size(2) == dim, "rotary_append: pools must be [", hk, ", T, ", dim, "], got ",
+                    kp.sizes());
+  const at::ScalarType type = q.scalar_type();
+  TORCH_CHECK_VALUE(half_type(type) && k.scalar_type() == type && v.scalar_type() == type && kp.scalar_type() == type &&
+                        vp.scalar_type() == type,
+                    "rotary_append: q, k, v and the pools must share one dtype, bfloat16 or float16");
+  const int64_t rot = 2 * freq.numel();
+  TORCH_CHECK_VALUE(freq.scalar_type() == at::kFloat && freq.dim() == 1 && rot <= dim && rot % 16 == 0,
+                    "rotary_append: inv_freq must be float32 [rotary_dim / 2], rotary_dim a multiple of 16 up to D");
+  TORCH_CHECK_VALUE(positions.scalar_type() == at::kLong && positions.dim() == 1 && positions.size(0) == n,
+                    "rotary_append: positions must be int64 [N]");
+  TORCH_CHECK_VALUE(targets.scalar_type() == at::kLong && targets.dim() == 1 && targets.size(0) == n,
+                    "rotary_append: targets must be int64 [N]");
+  for (at::Tensor* w : {&qw, &kw}) {
+    if (!w->defined()) continue;
+    TORCH_CHECK_VALUE(w->scalar_type() == type && w->dim() == 1 && w->size(0) == dim,
+                      "rotary_append: norm weights must be [D] of the inputs' dtype");
+  }
+  check_status("rotary_append", status, device);
+  if (klen.defined()) {
+    TORCH_CHECK_VALUE(count.defined() && count.scalar_type() == at::kLong && count.numel() >= 1,
+                      "rotary_append: the step count must be an int64 tensor of at least one element on the pools' device");
+    TORCH_CHECK_VALUE(klen.scalar_type() == at::kInt && tails.defined() && tails.scalar_type() == at::kInt,
+                      "rotary_append: the cached plan's lengths and tail indices must be int32");
+  }
+  const c10::cuda::CUDAGuard guard(device);
+  q = rows16(q), k = rows16(k), v = rows16(v);
+  positions = packed(positions), targets = packed(targets), freq = packed(freq);
+  for (at::Tensor* w : {&qw, &kw})
+    if (w->defined() && !(w->is_contiguous() && aligned16(*w))) *w = w->clone(at::MemoryFormat::Contiguous);
+  if (!out.defined()) {
+    out = at::empty({n, hq, dim}, q.options());
+  } else {
+    TORCH_CHECK_VALUE(out.dim() == 3 && out.size(0) == n && out.size(1) == hq && out.size(2) == dim &&
+                          out.scalar_type() == type && out.is_contiguous() && aligned16(out),
+                      "rotary_append: out must be contiguous [N, HQ, D] of the inputs' dtype, 16-byte aligned");
+    const bool same = out.data_ptr() == q.data_ptr() && q.is_contiguous();
+    TORCH_CHECK_VALUE(!overlap(out, k) && !overlap(out, v) && !overlap(out, kp) && !overlap(out, vp) &&
+                          (same || !overlap(out, q)),
+                      "rotary_append: out overlaps an input");
+  }
+  done(entry.rotary_append(
+           q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+           v.stride(1), positions.data_ptr<int64_t>(), freq.data_ptr<float>(), int32_t(rot), interleaved, float(factor),
+           ptr(qw), ptr(kw), float(eps), out.data_ptr(), kp.data_ptr(), vp.data_ptr(), targets.data_ptr<int64_t>(),
+           narrow(n, "N"), narrow(hq, "HQ"), narrow(hk, "HK"), kp.size(1), int32_t(dim), dtype_code(type),
+           static_cast<int32_t*>(ptr(klen)), static_cast<const int32_t*>(ptr(tails)),
+           tails.defined() ? narrow(tails.numel(), "tails") : 0, static_cast<const int64_t*>(ptr(count)), offset, jobs,
+           static_cast<int32_t*>(ptr(status)), stream_of(device)),
+       "ta_rotary_append");
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* chunk_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  count_args(n_args, 12);
+  at::Tensor q = tensor(a[0], "q");
+  const at::Tensor &kp = tensor(a[1], "kp"), &vp = tensor(a[2], "vp"), &table = tensor(a[3], "table");
+  at::Tensor lens = tensor(a[4], "kv_lens"), cu = tensor(a[5], "cu_q");
+  const int64_t page = integer(a[6]);
+  TORCH_CHECK_VALUE(q.dim() == 3 && kp.dim() == 3, "q must be [N, HQ, D] and the pools [HK, T, D]");
+  const int64_t n = q.size(0), hq = q.size(1), dim = q.size(2), hk = kp.size(0);
+  const double scale = a[7] == Py_None ? 1.0 / std::sqrt(double(dim)) : real(a[7]);
+  const bool causal = truth(a[8]);
+  at::Tensor out = optional(a[9], "out");
+  const at::Tensor lse = optional(a[10], "out_lse"), status = optional(a[11], "status");
+
+  const at::Device device = q.device();
+  TORCH_CHECK_VALUE(q.is_cuda(), "chunk_attention: all tensors must be CUDA tensors on one device");
+  one_device("chunk_attention", device, {&kp, &vp, &table, &lens, &cu, &out, &lse});
+  check_pools("chunk_attention", kp, vp);
+  TORCH_CHECK_VALUE(head_dim_ok(dim) && kp.size(2) == dim,
+                    "chunk_attention: head_dim must be 32, 64 or 128 and that of the pools");
+  const at::ScalarType type = q.scalar_type();
+  TORCH_CHECK_VALUE(half_type(type) && kp.scalar_type() == type && vp.scalar_type() == type,
+                    "q, K and V must share one dtype, bfloat16 or float16");
+  TORCH_CHECK_VALUE(hk > 0 && hq > 0 && hq % hk == 0, "Query heads must be divisible by KV heads");
+  TORCH_CHECK_VALUE(page >= 1 && (page & (page - 1)) == 0, "chunk_attention: page_size must be a power of two");
+  const int64_t b = lens.dim() == 1 ? lens.size(0) : -1;
+  TORCH_CHECK_VALUE(b >= 0 && lens.scalar_type() == at::kInt && cu.scalar_type() == at::kInt && cu.dim() == 1 &&
+                        cu.size(0) == b + 1,
+                    "chunk_attention: kv_lens must be int32 [B] and cu_q int32 [B + 1]");
+  TORCH_CHECK_VALUE(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == b &&
+                        (table.size(1) <= 1 || table.stride(1) == 1),
+                    "chunk_attention: table must be int32 [B, W] with contiguous rows");
+  TORCH_CHECK_VALUE(float(scale) > 0 && std::isfinite(float(scale)), "chunk_attention: scale must be positive");
+  check_status("chunk_attention", status, device);
+  const c10::cuda::CUDAGuard guard(device);
+  q = rows16(q), lens = packed(lens), cu = packed(cu);
+  if (!out.defined()) {
+    out = at::empty({n, hq, dim}, q.options());
+  } else {
+    TORCH_CHECK_VALUE(out.dim() == 3 && out.size(0) == n && out.size(1) == hq && out.size(2) == dim &&
+                          out.scalar_type() == type && out.is_contiguous() && aligned16(out),
+                      "chunk_attention: out must be contiguous [N, HQ, D] like q, 16-byte aligned");
+    TORCH_CHECK_VALUE(!overlap(out, q) && !overlap(out, kp) && !overlap(out, vp), "chunk_attention: out overlaps an input");
+  }
+  TORCH_CHECK_VALUE(!lse.defined() || (lse.dim() == 2 && lse.size(0) == n && lse.size(1) == hq &&
+                                       lse.scalar_type() == at::kFloat && lse.is_contiguous()),
+                    "chunk_attention: out_lse must be contiguous float32 [N, HQ] on q's device");
+  if (n > 0 && b > 0) {
+    const int32_t tokens = narrow(n, "N"), seqs = narrow(b, "B"), heads = narrow(hq, "HQ"), width = narrow(table.size(1), "W"),
+                  rows = narrow(page, "page_size");
+    const int64_t bytes = entry.chunk_workspace_bytes(tokens, seqs, heads, int32_t(hk), int32_t(dim), width, rows);
+    at::Tensor workspace;
+    if (bytes) workspace = at::empty({bytes}, q.options().dtype(at::kByte));
+    done(entry.chunk_attention(q.data_ptr(), q.stride(0), q.stride(1), kp.data_ptr(), vp.data_ptr(), kp.size(1),
+                               table.data_ptr<int32_t>(), table.stride(0), width, rows, lens.data_ptr<int32_t>(),
+                               cu.data_ptr<int32_t>(), seqs, tokens, heads, int32_t(hk), int32_t(dim), dtype_code(type),
+                               float(scale), causal, out.data_ptr(), static_cast<float*>(ptr(lse)), ptr(workspace), bytes,
+                               static_cast<int32_t*>(ptr(status)), stream_of(device)),
+         "ta_chunk_attention");
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+constexpr int64_t kMaxBeams = 32, kMaxK = 32;
+
+PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  count_args(n_args, 5);
+  at::Tensor logits = tensor(a[0], "logits"), scores = tensor(a[1], "scores");
+  at::Tensor finished = optional(a[3], "finished");
+  const int64_t end = integer(a[4]);
+  TORCH_CHECK_VALUE(scores.dim() == 2 && scores.scalar_type() == at::kFloat, "beam_select: scores must be float32 [R, W]");
+  const int64_t r = scores.size(0), w = scores.size(1);
+  TORCH_CHECK_VALUE((logits.dim() == 3 && logits.size(0) == r && logits.size(1) == w) ||
+                        (logits.dim() == 2 && logits.size(0) == r * w),
+                    "beam_select: logits must be [R, W, V] or [R * W, V]");
+  const int64_t vocab = logits.size(-1), k = a[2] == Py_None ? w : integer(a[2]);
+  const at::Device device = logits.device();
+  TORCH_CHECK_VALUE(logits.is_cuda(), "beam_select: all tensors must be CUDA tensors on one device");
+  one_device("beam_select", device, {&scores, &finished});
+  const int32_t type = dtype_code(logits.scalar_type());
+  TORCH_CHECK_VALUE(type != 0, "beam_select: logits must be bfloat16, float16 or float32");
+  TORCH_CHECK_VALUE(w >= 1 && w <= kMaxBeams && k >= 1 && k <= kMaxK && vocab >= 1 && k <= w * vocab, "beam_select: 1 to ",
+                    kMaxBeams, " beams, k from 1 to ", kMaxK, " and at most W * V");
+  if (finished.defined()) {
+    TORCH_CHECK_VALUE(finished.scalar_type() == at::kBool && finished.sizes() == scores.sizes(),
+                      "beam_select: finished must be bool [R, W]");
+    TORCH_CHECK_VALUE(end >= 0 && end < vocab, "beam_select: finished beams need an end_token within the vocabulary");
+  }
+  const c10::cuda::CUDAGuard guard(device);
+  if (finished.defined()) finished = packed(finished);
+  scores = packed(scores);
+  // one stride between beam rows
+  if ((vocab > 1 && logits.stride(-1) != 1) ||
+      (logits.dim() == 3 && r > 1 && w > 1 && logits.stride(0) != w * logits.stride(1)))
+    logits = logits.contiguous();
+  const int64_t stride = logits.stride(logits.dim() == 3 && w == 1 ? 0 : logits.dim() - 2);
+  at::Tensor best = at::empty({r, k}, scores.options());
+  const at::Tensor chosen = at::empty({2, r, k}, scores.options().dtype(at::kLong));
+  at::Tensor parents = chosen.select(0, 0), tokens = chosen.select(0, 1);
+  if (r > 0) {
+    const int32_t requests = narrow(r, "R"), words = narrow(vocab, "V");
+    const int64_t bytes = entry.beam_workspace_bytes(requests, int32_t(w), words, int32_t(k), type);
+    const at::Tensor workspace = at::empty({bytes}, scores.options().dtype(at::kByte));
+    done(entry.beam_select(logits.data_ptr(), stride, scores.data_ptr<float>(), static_cast<const uint8_t*>(ptr(finished)),
+                           requests, int32_t(w), words, int32_t(k), narrow(end, "end_token"), type, best.data_ptr<float>(),
+                           parents.data_ptr<int64_t>(), tokens.data_ptr<int64_t>(), workspace.data_ptr(), bytes,
+                           stream_of(device)),
+         "ta_beam_select");
+  }
+  THPObjectPtr tuple(PyTuple_New(3));
+  if (!tuple) throw python_error();
+  PyTuple_SET_ITEM(tuple.get(), 0, THPVariable_Wrap(std::move(best)));
+  PyTuple_SET_ITEM(tuple.get(), 1, THPVariable_Wrap(std::move(parents)));
+  PyTuple_SET_ITEM(tuple.get(), 2, THPVariable_Wrap(std::move(tokens)));
+  return tuple.release();
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  count_args(n_args, 4);
+  at::Tensor states = tensor(a[0], "states"), parents = tensor(a[1], "parents"), out = optional(a[2], "out");
+  const at::Tensor status = optional(a[3], "status");
+  TORCH_CHECK_VALUE(states.dim() >= 2 && parents.dim() == 2 && parents.size(0) == states.size(0),
+                    "beam_reorder wants states [R, W, ...] and parents [R, K]");
+  TORCH_CHECK_VALUE(parents.scalar_type() == at::kLong, "beam_reorder: parents must be int64");
+  const at::Device device = states.device();
+  TORCH_CHECK_VALUE(states.is_cuda(), "beam_reorder: all tensors must be CUDA tensors on one device");
+  one_device("beam_reorder", device, {&parents, &out});
+  check_status("beam_reorder", status, device);
+  const int64_t r = states.size(0), w = states.size(1), kept = parents.size(1);
+  TORCH_CHECK_VALUE(w > 0 || r * kept == 0, "beam_reorder: no beams to take rows from");
+  const c10::cuda::CUDAGuard guard(device);
+  // the rows themselves have to be contiguous
+  int64_t expected = 1;
+  bool whole = true;
+  for (int64_t i = states.dim() - 1; i >= 2; --i) {
+    whole &= states.size(i) == 1 || states.stride(i) == expected;
+    expected *= states.size(i);
+  }
+  if (!whole) states = states.contiguous();
+  if (kept > 1 && parents.stride(1) != 1) parents = parents.contiguous();
+  at::DimVector shape(states.sizes().begin(), states.sizes().end());
+  shape[1] = kept;
+  if (!out.defined()) {
+    out = at::empty(shape, states.options());
+  } else {
+    TORCH_CHECK_VALUE(out.sizes() == at::IntArrayRef(shape) && out.scalar_type() == states.scalar_type() && out.is_contiguous(),
+                      "beam_reorder: out must be contiguous [R, K, ...] of the states' dtype");
+    TORCH_CHECK_VALUE(!overlap(out, states) && !overlap(out, parents), "beam_reorder: out overlaps an input");
+  }
+  if (out.numel() > 0) {
+    const int64_t size = states.element_size();
+    done(entry.beam_reorder(states.data_ptr(), states.stride(0) * size, states.stride(1) * size, narrow(r, "R"),
+                            narrow(w, "W"), expected * size, parents.data_ptr<int64_t>(), parents.stride(0),
+                            narrow(kept, "K"), out.data_ptr(), static_cast<int32_t*>(ptr(status)), stream_of(device)),
+         "ta_beam_reorder");
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// bind(addresses): the entry points in the order of struct Entry.
+PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  constexpr Py_ssize_t kEntries = sizeof(Entry) / sizeof(void*);
+  count_args(n_args, kEntries);
+  void* address[kEntries];
+  for (Py_ssize_t i = 0; i < kEntries; ++i) {
+    address[i] = PyLong_AsVoidPtr(a[i]);
+    if (!address[i]) {
+      if (PyErr_Occurred()) throw python_error();
+      TORCH_CHECK_VALUE(false, "null entry point");
+    }
+  }
+  static_assert(sizeof(address) == sizeof(Entry), "one pointer an entry point");
+  std::memcpy(&entry, address, sizeof(Entry));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef methods[] = {
+    {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
+    {"rotary_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary_append)), METH_FASTCALL, nullptr},
+    {"chunk_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(chunk_attention)), METH_FASTCALL, nullptr},
+    {"beam_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(beam_select)), METH_FASTCALL, nullptr},
+    {"beam_reorder", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(beam_reorder)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__ops() { return PyModule_Create(&module); }

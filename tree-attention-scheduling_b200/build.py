@@ -1,7 +1,8 @@
-"""Build the sm_100a kernel library in-tree: ``tree_attention/libtree_attn_b200.so``.
+"""Build the sm_100a kernel library in-tree: ``tree_attention/libtree_attn_b200.so``, and the operators' Python calls.
 
 Plain ``nvcc -shared`` over ``csrc/*.cu`` and the host-only ``csrc/*.cpp`` (static CUDA runtime, so the library
 is self-contained behind its C ABI; streams are passed in as cudaStream_t).
+``build_binding()`` compiles ``binding/ops.cpp`` against the installed torch into ``tree_attention/_ops.so``.
 Run ``python build.py`` or call ``build()``; rebuilds only when a source or the
 public header is newer than the library.
 """
@@ -18,6 +19,8 @@ REPO = HERE.parent
 CSRC = HERE / "csrc"
 INCLUDE = REPO / "include"
 LIB = HERE / "tree_attention" / "libtree_attn_b200.so"
+BINDING = HERE / "binding" / "ops.cpp"
+OPS = HERE / "tree_attention" / "_ops.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -72,5 +75,29 @@ def build(force=False, verbose=False, extra_flags=()):
     return LIB
 
 
+def build_binding(force=False, verbose=False):
+    """Compile the operators' Python calls against the installed torch: ``tree_attention/_ops.so``."""
+    deps = [BINDING, *INCLUDE.glob("*.h"), Path(__file__)]
+    if not force and OPS.exists() and all(p.stat().st_mtime <= OPS.stat().st_mtime for p in deps):
+        return OPS
+    import sysconfig
+
+    import torch
+    base = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc_path()).resolve().parents[1]
+    includes = [INCLUDE, base / "include", base / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
+                sysconfig.get_paths()["include"]]
+    tmp = OPS.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in includes), str(BINDING),
+           "-o", str(tmp), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, OPS)
+    return OPS
+
+
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose=True))
+    print(build_binding(force="--force" in sys.argv, verbose=True))

@@ -125,6 +125,31 @@ def load():
     return lib
 
 
+_ops = None
+
+
+def ops():
+    """The operators' Python calls (``_ops.so``, built by ``build.py``), bound to the loaded kernel library.
+
+    They check arguments, make outputs and workspaces and launch in C++: a
+    fifth of the host time of the same through ctypes.
+    """
+    global _ops
+    if _ops is None:
+        lib = load()
+        import torch  # noqa: F401  (its libraries first)
+        try:
+            from . import _ops as module
+        except ImportError as e:
+            raise RuntimeError(f"tree-attention binding not usable ({e}); "
+                               "build it with `python tree-attention-scheduling_b200/build.py`") from e
+        module.bind(*[ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "ta_error_string", "ta_rotary_append", "ta_chunk_workspace_bytes", "ta_chunk_attention",
+            "ta_beam_workspace_bytes", "ta_beam_select", "ta_beam_reorder")])
+        _ops = module
+    return _ops
+
+
 def check(rc, what):
     if rc != 0:
         raise RuntimeError(f"{what} failed: {describe_status(rc)} (code {rc})")

@@ -16,10 +16,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from . import _lib
-from ._launch import DTYPES, check_pools, check_status_tensor, launch, overlap, ptr, rows16
-
-HEAD_DIMS = (32, 64, 128)
+from ._lib import ops
 
 
 def path_table(paths, device):
@@ -51,62 +48,4 @@ def chunk_attention(q, kp, vp, table, kv_lens, cu_q, page_size=1, scale=None, ca
     Lengths beyond the table and positions outside the pools are recorded in
     ``status`` (int32, one element) and not followed.
     """
-    if q.dim() != 3 or kp.dim() != 3:
-        raise ValueError("q must be [N, HQ, D] and the pools [HK, T, D]")
-    n, hq, dim = q.shape
-    device, dtype = q.device, q.dtype
-    if not q.is_cuda:
-        raise ValueError("chunk_attention: all tensors must be CUDA tensors on one device")
-    check_pools("chunk_attention", kp, vp, device)
-    hk, tokens, kdim = kp.shape
-    if dim not in HEAD_DIMS or kdim != dim:
-        raise ValueError(f"chunk_attention: head_dim must be one of {HEAD_DIMS} and that of the pools")
-    if dtype not in DTYPES or kp.dtype != dtype or vp.dtype != dtype:
-        raise ValueError("q, K and V must share one dtype, bfloat16 or float16")
-    if hk == 0 or hq == 0 or hq % hk:
-        raise ValueError("Query heads must be divisible by KV heads")
-    if page_size < 1 or page_size & (page_size - 1):
-        raise ValueError("chunk_attention: page_size must be a power of two")
-    b = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
-    if kv_lens.dtype != torch.int32 or b < 0 or cu_q.dtype != torch.int32 or cu_q.shape != (b + 1,):
-        raise ValueError("chunk_attention: kv_lens must be int32 [B] and cu_q int32 [B + 1]")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != b or (table.shape[1] > 1
-                                                                                  and table.stride(1) != 1):
-        raise ValueError("chunk_attention: table must be int32 [B, W] with contiguous rows")
-    if any(t.device != device for t in (table, kv_lens, cu_q)):
-        raise ValueError("chunk_attention: all tensors must be CUDA tensors on one device")
-    if scale is None:
-        scale = dim ** -0.5
-    elif not (scale > 0 and scale < float("inf")):
-        raise ValueError("chunk_attention: scale must be positive")
-    check_status_tensor("chunk_attention", status, device)
-    q = rows16(q)
-    kv_lens, cu_q = kv_lens.contiguous(), cu_q.contiguous()
-    if out is None:
-        out = torch.empty((n, hq, dim), device=device, dtype=dtype)
-    elif out.shape != (n, hq, dim) or out.dtype != dtype or out.device != device or not out.is_contiguous() \
-            or out.data_ptr() % 16:
-        raise ValueError("chunk_attention: out must be contiguous [N, HQ, D] like q, 16-byte aligned")
-    elif any(overlap(out, t) for t in (q, kp, vp)):
-        raise ValueError("chunk_attention: out overlaps an input")
-    if out_lse is not None and (out_lse.shape != (n, hq) or out_lse.dtype != torch.float32
-                                or out_lse.device != device or not out_lse.is_contiguous()):
-        raise ValueError("chunk_attention: out_lse must be contiguous float32 [N, HQ] on q's device")
-    if n == 0 or b == 0:
-        return out
-    width = table.shape[1]
-    workspace, size = None, _workspace_bytes(device, n, b, hq, hk, dim, width, page_size)
-    if size:
-        workspace = torch.empty(size, device=device, dtype=torch.uint8)
-    launch("ta_chunk_attention", device, q.data_ptr(), q.stride(0), q.stride(1), kp.data_ptr(), vp.data_ptr(), tokens,
-           table.data_ptr(), table.stride(0), width, page_size, kv_lens.data_ptr(), cu_q.data_ptr(), b, n, hq, hk, dim,
-           DTYPES[dtype], scale, int(causal), out.data_ptr(), ptr(out_lse), ptr(workspace), size, ptr(status))
-    return out
-
-
-def _workspace_bytes(device, *sizes):
-    lib = _lib.load()
-    if device.index == torch.cuda.current_device():
-        return lib.ta_chunk_workspace_bytes(*sizes)
-    with torch.cuda.device(device.index):
-        return lib.ta_chunk_workspace_bytes(*sizes)
+    return ops().chunk_attention(q, kp, vp, table, kv_lens, cu_q, page_size, scale, causal, out, out_lse, status)

@@ -14,9 +14,7 @@ import math
 
 import torch
 
-from ._launch import DTYPES, check_pools, check_status_tensor, launch, overlap, ptr, rows16
-
-HEAD_DIMS = (32, 64, 128)
+from ._lib import ops
 
 
 def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, length=None, device=None):
@@ -102,61 +100,12 @@ def rotary_append(q, k, v, positions, inv_freq, kp, vp, targets, interleaved=Fal
     lengths, as in ``append_kv``.  ``out`` may be ``q`` itself where that is
     contiguous.
     """
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
-        raise ValueError("rotary_append wants q [N, HQ, D] and k, v [N, HK, D]")
-    n, hq, dim = q.shape
-    hk = k.shape[1]
-    device = q.device
-    if not q.is_cuda:
-        raise ValueError("rotary_append: all tensors must be CUDA tensors on one device")
-    if dim not in HEAD_DIMS:
-        raise ValueError(f"rotary_append: head_dim must be one of {HEAD_DIMS}")
-    check_pools("rotary_append", kp, vp, device)
-    if kp.shape[0] != hk or kp.shape[2] != dim:
-        raise ValueError(f"rotary_append: pools must be [{hk}, T, {dim}], got {tuple(kp.shape)}")
-    dtype = q.dtype
-    if dtype not in DTYPES or any(t.dtype != dtype for t in (k, v, kp, vp)):
-        raise ValueError("rotary_append: q, k, v and the pools must share one dtype, bfloat16 or float16")
-    rot = 2 * inv_freq.numel()
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or rot > dim or rot % 16:
-        raise ValueError("rotary_append: inv_freq must be float32 [rotary_dim / 2], rotary_dim a multiple of 16 up to D")
-    for name, t in (("positions", positions), ("targets", targets)):
-        if t.dtype != torch.int64 or t.shape != (n,):
-            raise ValueError(f"rotary_append: {name} must be int64 [N]")
-    for w in (q_weight, k_weight):
-        if w is not None and (w.dtype != dtype or w.shape != (dim,)):
-            raise ValueError("rotary_append: norm weights must be [D] of the inputs' dtype")
-    if any(t is not None and t.device != device for t in (k, v, positions, inv_freq, targets, q_weight, k_weight, out)):
-        raise ValueError("rotary_append: all tensors must be CUDA tensors on one device")
-    check_status_tensor("rotary_append", status, device)
-    q, k, v = rows16(q), rows16(k), rows16(v)
-    positions, targets, inv_freq = positions.contiguous(), targets.contiguous(), inv_freq.contiguous()
-    q_weight, k_weight = (w if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0)
-                          else w.clone(memory_format=torch.contiguous_format) for w in (q_weight, k_weight))
-    if out is None:
-        out = torch.empty((n, hq, dim), device=device, dtype=dtype)
-    else:
-        if out.shape != (n, hq, dim) or out.dtype != dtype or not out.is_contiguous() or out.data_ptr() % 16:
-            raise ValueError("rotary_append: out must be contiguous [N, HQ, D] of the inputs' dtype, 16-byte aligned")
-        same = out.data_ptr() == q.data_ptr() and q.is_contiguous()
-        if any(overlap(out, t) for t in (k, v, kp, vp)) or (overlap(out, q) and not same):
-            raise ValueError("rotary_append: out overlaps an input")
     klen = tail_ids = count = None
-    offset = num_tails = num_jobs = 0
+    offset = num_jobs = 0
     if tails is not None:
-        cached, count_t, offset = tails
+        cached, count, offset = tails
         p = cached.prepared
-        if count_t.device != device or count_t.dtype != torch.int64 or count_t.numel() < 1:
-            raise ValueError("rotary_append: the step count must be an int64 tensor of at least one element "
-                             "on the pools' device")
-        if p.klen.device != device or cached.tail_indices.device != device or cached.tail_indices.dtype != torch.int32:
-            raise ValueError("rotary_append: the cached plan lives on another device than the pools")
-        klen, tail_ids, count = p.klen.data_ptr(), cached.tail_indices.data_ptr(), count_t.data_ptr()
-        num_tails, num_jobs = cached.tail_indices.numel(), p.layout.num_jobs
+        klen, tail_ids, num_jobs = p.klen, cached.tail_indices, p.layout.num_jobs
         status = p.status if status is None else status
-    launch("ta_rotary_append", device, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-           v.data_ptr(), v.stride(0), v.stride(1), positions.data_ptr(), inv_freq.data_ptr(), rot, int(interleaved),
-           float(attention_factor), ptr(q_weight), ptr(k_weight), float(eps), out.data_ptr(), kp.data_ptr(),
-           vp.data_ptr(), targets.data_ptr(), n, hq, hk, kp.shape[1], dim, DTYPES[dtype], klen, tail_ids, num_tails,
-           count, int(offset), num_jobs, ptr(status))
-    return out
+    return ops().rotary_append(q, k, v, positions, inv_freq, kp, vp, targets, interleaved, attention_factor, q_weight,
+                               k_weight, eps, out, status, klen, tail_ids, count, offset, num_jobs)
