@@ -1,0 +1,202 @@
+"""The decoder's paths over the operators: chunked prefill, fused rotary decode, beam search.
+
+On CPU the operators' plain forms stand in (module globals of the adapter, as the
+attention stand-in of the other adapter tests); on a B200 the kernels run.
+Logits are compared with full-sequence forwards of the same model.  In float32
+the two differ by summation order alone (1e-4 as in the other adapter tests); in
+float16 by the rounding of activations, for which those tests' 4e-3 / 2e-2 hold.
+A sum of T log-probabilities of such logits is off by at most T times twice a
+logit's tolerance.
+"""
+import pytest
+import torch
+
+from tree_attention import CostModel, qwen
+
+transformers = pytest.importorskip("transformers")
+from tests.test_qwen import (SEQUENCES, oracle_attention, reference_append, reference_logits,  # noqa: E402
+                             tiny_model)
+
+TREES = [SEQUENCES, [[5, 6, 7]], [[1], [2, 3], [1, 4]],
+         [[9, 8, 7, 6, 5, 4, 3], [9, 8, 7, 6, 5], [9, 8, 7, 6, 5, 4, 3, 2, 1, 0], [1, 1]]]
+
+
+# ---- plain forms ------------------------------------------------------------------
+def plain_rotary(q, k, v, positions, inv_freq, kp, vp, targets, interleaved=False, attention_factor=1.0,
+                 q_weight=None, k_weight=None, eps=1e-6, out=None, status=None, tails=None):
+    angle = positions.double()[:, None] * inv_freq.double()
+    cos, sin = (f(angle)[:, None] * attention_factor for f in (torch.cos, torch.sin))
+    half = inv_freq.numel()
+
+    def turn(x, weight):
+        y = x.double()
+        y = y / (y.square().mean(-1, keepdim=True) + eps).sqrt() * weight.double()
+        a, b = y[..., :half], y[..., half:2 * half]
+        return torch.cat((a * cos - b * sin, b * cos + a * sin, y[..., 2 * half:]), -1).to(x.dtype)
+
+    kp[:, targets] = turn(k, k_weight).transpose(0, 1)
+    vp[:, targets] = v.transpose(0, 1)
+    return turn(q, q_weight)
+
+
+def plain_chunk(q, kp, vp, table, kv_lens, cu_q, page_size=1, scale=None, causal=True, out=None, out_lse=None,
+                status=None):
+    group = q.shape[1] // kp.shape[0]
+    result = torch.zeros_like(q)
+    for b, keys in enumerate(kv_lens.tolist()):
+        first, last = cu_q[b].item(), cu_q[b + 1].item()
+        path = table[b, :keys].long()
+        k, v = (x[:, path].repeat_interleave(group, 0).double() for x in (kp, vp))
+        s = torch.einsum("nhd,hkd->hnk", q[first:last].double(), k) * scale
+        hidden = torch.arange(keys) > keys - (last - first) + torch.arange(last - first)[:, None]
+        result[first:last] = torch.einsum("hnk,hkd->nhd", s.masked_fill(hidden, -torch.inf).softmax(-1), v).to(q.dtype)
+    return result
+
+
+def plain_select(logits, scores, k=None, finished=None, end_token=-1):
+    x = logits.double().log_softmax(-1) + scores.double()[..., None]
+    if finished is not None:
+        ended = torch.where(torch.arange(x.shape[-1]) == end_token, scores.double()[..., None], -torch.inf)
+        x = torch.where(finished[..., None], ended, x)
+    best, index = x.flatten(1).sort(dim=1, descending=True, stable=True)
+    index = index[:, :k]
+    return best[:, :k].float(), index // x.shape[-1], index % x.shape[-1]
+
+
+def plain_reorder(states, parents, out=None, status=None):
+    return torch.stack([s[p] for s, p in zip(states, parents)])
+
+
+@pytest.fixture
+def plain(monkeypatch):
+    monkeypatch.setattr(qwen, "rotary_append", plain_rotary)
+    monkeypatch.setattr(qwen, "chunk_attention", plain_chunk)
+    monkeypatch.setattr(qwen, "beam_select", plain_select)
+    monkeypatch.setattr(qwen, "beam_reorder", plain_reorder)
+    monkeypatch.setattr(qwen, "append_kv", reference_append)
+    return monkeypatch
+
+
+def searched(model, sequence, steps, beams, end):
+    """Beam search of one prompt by full forwards, 64-bit scores: (tokens, score) best first."""
+    kept = [([], 0.0)]
+    for _ in range(steps):
+        candidates = []
+        for b, (tokens, score) in enumerate(kept):
+            if end is not None and tokens and tokens[-1] == end:
+                candidates.append((score, -b, -end, tokens + [end]))
+                continue
+            logits = reference_logits(model, [sequence + tokens])[0].double().log_softmax(-1)
+            best = logits.topk(min(beams, len(logits)))
+            candidates += [(score + x, -b, -i, tokens + [i]) for x, i in zip(best[0].tolist(), best[1].tolist())]
+        kept = [(c[3], c[0]) for c in sorted(candidates, reverse=True)[:beams]]
+    return kept
+
+
+# ---- on the CPU ----------------------------------------------------------------------
+@pytest.mark.parametrize("chunk_tokens", [1, 3, 8192])
+@pytest.mark.parametrize("sequences", TREES, ids=["five", "one", "short", "nested"])
+def test_chunked_prefill_fills_the_pools(sequences, chunk_tokens, plain):
+    model = tiny_model(32, 4, 2, torch.float32, "cpu")
+    a = qwen.SharedKVDecoder(model, sequences, max_new_tokens=2, prefill="chunked", chunk_tokens=chunk_tokens)
+    b = qwen.SharedKVDecoder(model, sequences, max_new_tokens=2, prefill="per_request")
+    n = a.prefix_size
+    for (ka, va), (kb, vb) in zip(a.pools, b.pools):
+        torch.testing.assert_close(ka[:, :n], kb[:, :n], atol=1e-4, rtol=1e-4)
+        torch.testing.assert_close(va[:, :n], vb[:, :n], atol=1e-4, rtol=1e-4)
+    torch.testing.assert_close(a.logits, reference_logits(model, sequences), atol=1e-4, rtol=1e-4)
+
+
+@pytest.mark.parametrize("cached", [False, True])
+def test_fused_rotary_steps_match_full_forward(cached, plain):
+    model = tiny_model(32, 4, 2, torch.float32, "cpu")
+    cls = qwen.CachedPrefixDecoder if cached else qwen.SharedKVDecoder
+    if cached:
+        plain.setattr(qwen.CachedDecodePlan, "update", lambda self, n: self.prepared)
+    decoder = cls(model, SEQUENCES, max_new_tokens=4, prefill="chunked", rotary="fused")
+    plain.setattr(qwen, "attention_matrix", oracle_attention(decoder))
+    for _ in range(3):
+        logits = decoder.step(decoder.logits.argmax(-1).tolist())
+        torch.testing.assert_close(logits, reference_logits(model, decoder.sequences), atol=1e-4, rtol=1e-4)
+
+
+@pytest.mark.parametrize("end", [None, 57])
+def test_beam_search_equals_full_forwards(end, plain):
+    model = tiny_model(32, 4, 2, torch.float32, "cpu")
+    decoder = qwen.SharedKVDecoder(model, SEQUENCES, max_new_tokens=5, prefill="chunked", beams=4)
+    if end is not None:                                      # a token that some beams take
+        end = decoder.logits[0].topk(3)[1][2].item()
+    for beams in (1, 3, 4):
+        tokens, scores = decoder.beam_search(4, beams, end)
+        assert tokens.shape == (len(SEQUENCES), beams, 4) and scores.shape == tokens.shape[:2]
+        for r, sequence in enumerate(SEQUENCES):
+            want = searched(model, sequence, 4, beams, end)
+            torch.testing.assert_close(scores[r], torch.tensor([s for _, s in want]), atol=1e-3, rtol=0)
+            assert tokens[r].tolist() == [t for t, _ in want]
+    # the decoder goes on from its prompts
+    plain.setattr(qwen, "attention_matrix", oracle_attention(decoder))
+    logits = decoder.step(decoder.logits.argmax(-1).tolist())
+    torch.testing.assert_close(logits, reference_logits(model, decoder.sequences), atol=1e-4, rtol=1e-4)
+    with pytest.raises(ValueError):                          # not from the prompts any more
+        decoder.beam_search(2)
+
+
+def test_refusals(plain):
+    model = tiny_model(32, 4, 2, torch.float32, "cpu")
+    for bad in (dict(rotary="nope"), dict(beams=0), dict(chunk_tokens=0)):
+        with pytest.raises(ValueError):
+            qwen.SharedKVDecoder(model, SEQUENCES, **bad)
+    decoder = qwen.SharedKVDecoder(model, SEQUENCES, max_new_tokens=3, prefill="chunked", beams=2)
+    for args in ((4, 2), (0, 2), (2, 3), (2, 0)):
+        with pytest.raises(ValueError):
+            decoder.beam_search(*args)
+
+
+# ---- on the GPU ----------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(32, 4, 2), (64, 6, 2), (128, 8, 2)], ids=["d32", "d64", "d128"])
+def test_chunked_prefill_and_fused_decode_gpu(shape):
+    """Prompts of several key tiles in one and in many chunks, then eager and graph-captured fused steps."""
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    model = tiny_model(*shape, torch.float16, "cuda")
+    sequences = [s * 60 for s in SEQUENCES]
+    for chunk_tokens in (100, 8192):
+        decoder = qwen.CachedPrefixDecoder(model, sequences, max_new_tokens=8, cost_model=CostModel.b200(),
+                                           prefill="chunked", rotary="fused", chunk_tokens=chunk_tokens)
+        torch.testing.assert_close(decoder.logits.float(), reference_logits(model, sequences).float(), atol=4e-3, rtol=2e-2)
+        for _ in range(2):
+            logits = decoder.step(decoder.logits.argmax(-1).tolist())
+            torch.testing.assert_close(logits.float(), reference_logits(model, decoder.sequences).float(), atol=4e-3,
+                                       rtol=2e-2)
+        decoder.generate(4)
+        assert int(decoder.cached_plan.prepared.status) == 0
+        torch.testing.assert_close(decoder.logits.float(), reference_logits(model, decoder.sequences).float(), atol=4e-3,
+                                   rtol=2e-2)
+
+
+@pytest.mark.gpu
+def test_beam_search_gpu():
+    """Chunked prefill, then every operator together: scores are those of full forwards of the returned
+    tokens, best first, and one beam is the greedy continuation's score."""
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    model = tiny_model(128, 8, 2, torch.float16, "cuda")
+    sequences = [s * 40 for s in SEQUENCES]
+    decoder = qwen.CachedPrefixDecoder(model, sequences, max_new_tokens=6, cost_model=CostModel.b200(),
+                                       prefill="chunked", rotary="fused", beams=4)
+    steps, end = 6, int(decoder.logits[0].topk(2)[1][1])
+    for beams, stop in ((4, None), (4, end), (1, None)):
+        tokens, scores = decoder.beam_search(steps, beams, stop)
+        assert torch.all(scores[:, :-1] >= scores[:, 1:])
+        for r, sequence in enumerate(sequences):
+            assert len({tuple(t) for t in tokens[r].tolist()}) == beams
+            for path, score in zip(tokens[r].tolist(), scores[r].tolist()):
+                with torch.inference_mode():
+                    logits = model(torch.tensor([sequence + path], device="cuda"), use_cache=False).logits[0]
+                each = logits[len(sequence) - 1:-1].double().log_softmax(-1).gather(1, torch.tensor(path).cuda()[:, None])
+                taken = path.index(stop) + 1 if stop in path else steps
+                assert path[taken:] == [stop] * (steps - taken)
+                # a logit's tolerance, for the token and for the sum over the vocabulary
+                tol = sum(2 * (4e-3 + 2e-2 * float(row.abs().max())) for row in logits[len(sequence) - 1:-1].float())
+                assert abs(float(each[:taken].sum()) - score) <= tol

@@ -18,7 +18,16 @@ Differences from the reference, on purpose:
   the node's tokens with its ancestors' K/V as the attention cache, instead of
   one full forward per request (``prefill="per_request"`` is the reference's
   procedure, ``qwen.py:34-51``); logits of a request are those at the last
-  token of its terminal node;
+  token of its terminal node; ``prefill="chunked"`` runs the same tree straight
+  over the pools -- ragged batches of up to ``chunk_tokens`` tokens of nodes whose
+  ancestors are done, each layer one ``rotary_append`` and one ``chunk_attention``
+  over the nodes' paths, no cache besides the pools, logits of the terminal
+  tokens alone;
+* ``rotary="fused"`` lets a decode step's q/k norms, rotary embedding and append
+  run as one ``rotary_append`` launch a layer (f32 arithmetic, one rounding;
+  ``"model"``, the default, runs the model's own modules and ``append_kv``);
+* ``beam_search(steps, beams)`` searches continuations of every prompt, the beams'
+  shared pasts held once in the pools;
 * ``shard=(rank, world, group)`` splits the KV heads over GPUs (each rank owns
   ``HK / world`` KV heads and their query heads, the matching slices of the
   q/k/v projections and its slice of every pool) and all-gathers the attention
@@ -31,7 +40,10 @@ from types import MethodType
 
 import torch
 
+from .beam import beam_reorder, beam_select
+from .chunk import chunk_attention, path_table
 from .kernels import CachedDecodePlan, append_kv, attention_matrix, prepare
+from .rotary import rotary_append
 from .schedule import CostModel, schedule
 from .tree import KVTree
 
@@ -57,9 +69,13 @@ class SharedKVDecoder:
     """Qwen3 decode with one physical shared-prefix KV pool per layer (reference qwen.py:9-103)."""
 
     def __init__(self, model, sequences, max_new_tokens=32, method="cube", cost_model=None, prefill="shared",
-                 shard=None):
-        if prefill not in ("shared", "per_request"):
+                 shard=None, rotary="model", beams=1, chunk_tokens=8192):
+        if prefill not in ("shared", "per_request", "chunked"):
             raise ValueError(f"unknown prefill {prefill!r}")
+        if rotary not in ("model", "fused"):
+            raise ValueError(f"unknown rotary {rotary!r}")
+        if beams < 1 or chunk_tokens < 1:
+            raise ValueError("beams and chunk_tokens must be positive")
         self.model = model
         self.sequences = [list(s) for s in sequences]
         if not self.sequences or any(not s for s in self.sequences):
@@ -78,7 +94,9 @@ class SharedKVDecoder:
         self.local_hq = self.hq // self.world
         self.original = [layer.self_attn.forward for layer in model.model.layers]
         self.max_new_tokens = max_new_tokens
-        self.capacity = self.tree.storage_tokens + len(self.sequences) * max_new_tokens
+        self.rotary = rotary
+        self.beams = beams                                # beams the pools have room for (beam_search)
+        self.capacity = self.tree.storage_tokens + len(self.sequences) * max_new_tokens * beams
         self.used = self.tree.storage_tokens
         self.prefix_size = self.used
         self.generated = 0
@@ -88,8 +106,12 @@ class SharedKVDecoder:
         self.leaves = [next(i for i, n in enumerate(self.tree.nodes) if r in n.terminal)
                        for r in range(len(self.sequences))]
         self._slices = self._projection_slices()
+        # in float32, as the embedding itself computes, whatever type the model was cast to
+        self._inv_freq = model.model.rotary_emb.inv_freq.float()
         if prefill == "shared":
             self._prefill_shared()
+        elif prefill == "chunked":
+            self._prefill_chunked(chunk_tokens)
         else:
             self._prefill_per_request()
 
@@ -174,6 +196,97 @@ class SharedKVDecoder:
                     a = nodes[a].parent
         self.logits = torch.stack([node_logits[leaf] for leaf in self.leaves])
 
+    @torch.inference_mode()
+    def _prefill_chunked(self, chunk_tokens):
+        """Every tree node once, in ragged batches over the pools themselves.
+
+        A batch takes up to ``chunk_tokens`` tokens from nodes whose ancestors
+        are done, several nodes side by side or a part of a long one; the new
+        rows go to their positions and attend their paths so far.
+        """
+        nodes, node_logits = self.tree.nodes, {}
+        paths = {0: ()}                                   # positions of a node's ancestors
+        done = [0] * len(nodes)
+        ready = [0]
+        while ready:
+            batch, room = [], chunk_tokens
+            for i in ready:
+                take = min(len(nodes[i].tokens) - done[i], room)
+                if take or not nodes[i].tokens:
+                    batch.append((i, done[i], take))
+                    room -= take
+                if not room:
+                    break
+            work = [(i, start, take) for i, start, take in batch if take]
+            if work:
+                positions, targets, seen, last = [], [], [], []
+                for i, start, take in work:
+                    own = nodes[i].tokens
+                    positions.extend(range(len(paths[i]) + start, len(paths[i]) + start + take))
+                    targets.extend(own[start:start + take])
+                    seen.append(paths[i] + own[:start + take])
+                    if start + take == len(own) and nodes[i].terminal:
+                        last.append((i, len(targets) - 1))
+                hidden = self._run_chunks([self.tree.token_ids[p] for p in targets], positions, targets,
+                                          [take for _, _, take in work], path_table(seen, self.device))
+                if last:
+                    rows = torch.tensor([row for _, row in last], device=self.device)
+                    for (i, _), logits in zip(last, self.model.lm_head(hidden[rows])):
+                        node_logits[i] = logits
+            for i, start, take in batch:
+                done[i] = start + take
+                if done[i] == len(nodes[i].tokens):
+                    ready.remove(i)
+                    for child in nodes[i].children:
+                        paths[child] = paths[i] + nodes[i].tokens
+                    ready.extend(nodes[i].children)
+                    del paths[i]
+        self.logits = torch.stack([node_logits[leaf] for leaf in self.leaves])
+
+    def _run_chunks(self, tokens, positions, targets, counts, table):
+        """Final hidden states ``[N, hidden]`` of a ragged batch of new tokens (lists), their K/V at ``targets``."""
+        device = self.device
+        as_row = dict(device=device, dtype=torch.int64)
+        tokens, positions, targets = (torch.as_tensor(x, **as_row) for x in (tokens, positions, targets))
+        cu = torch.tensor([0] + counts, device=device).cumsum(0).to(torch.int32)
+        return self._run_rows(tokens, positions, targets, *table, cu)
+
+    def _run_rows(self, tokens, positions, targets, table, kv_lens, cu_q):
+        """The model over rows ``[N]`` of new tokens whose sequences lie in the pools (device tensors throughout)."""
+        forward = self._rows_forward(positions, targets, table, kv_lens, cu_q)
+        for layer in self.model.model.layers:
+            layer.self_attn.forward = MethodType(forward, layer.self_attn)
+        try:
+            return self.model.model(tokens[None], position_ids=positions[None], use_cache=False,
+                                    attention_mask={"full_attention": None, "sliding_attention": None}
+                                    ).last_hidden_state[0]
+        finally:
+            for layer, original in zip(self.model.model.layers, self.original):
+                layer.self_attn.forward = original
+
+    def _rows_forward(self, positions, targets, table, kv_lens, cu_q):
+        """A layer's attention over rows of new tokens: projections, one fused norm, rotary and append, attention
+        over the sequences' positions."""
+        decoder, n = self, positions.shape[0]
+
+        def forward(module, hidden_states, position_embeddings, attention_mask=None, **kwargs):
+            q, k, v = (x.view(n, -1, module.head_dim) for x in decoder._project(module, hidden_states))
+            kp, vp = decoder.pools[module.layer_idx]
+            q = decoder._rotary(module, q, k, v, positions, targets, None, None)
+            result = decoder._gather(chunk_attention(q, kp, vp, table, kv_lens, cu_q, scale=module.scaling), n)
+            return module.o_proj(result.reshape(1, n, -1)), None
+
+        return forward
+
+    def _rotary(self, module, q, k, v, positions, targets, status, tails):
+        """q turned, k and v appended to the layer's pools, in one launch."""
+        embedding = self.model.model.rotary_emb
+        kp, vp = self.pools[module.layer_idx]
+        return rotary_append(q, k, v, positions, self._inv_freq, kp, vp, targets,
+                             attention_factor=embedding.attention_scaling, q_weight=module.q_norm.weight,
+                             k_weight=module.k_norm.weight, eps=module.q_norm.variance_epsilon, status=status,
+                             tails=tails)
+
     def _cache_layers(self, cache):
         """(keys, values) per layer of a transformers cache, [1, HK, T, D] each."""
         if hasattr(cache, "layers"):
@@ -187,6 +300,24 @@ class SharedKVDecoder:
         return states[self.rank * self.local_hk:(self.rank + 1) * self.local_hk]
 
     # -- decode -----------------------------------------------------------------
+    def _project(self, module, hidden_states):
+        """This rank's q, k and v projections."""
+        if self._slices is None:
+            return module.q_proj(hidden_states), module.k_proj(hidden_states), module.v_proj(hidden_states)
+        qs, ks = self._slices
+        return tuple(torch.nn.functional.linear(hidden_states, proj.weight[rows],
+                                                None if proj.bias is None else proj.bias[rows])
+                     for proj, rows in ((module.q_proj, qs), (module.k_proj, ks), (module.v_proj, ks)))
+
+    def _gather(self, result, n):
+        """All heads of ``[n, local heads, D]`` attention outputs."""
+        if self.world == 1:
+            return result
+        # rank-major concatenation along dim 0 (the form every backend accepts)
+        gathered = torch.empty((self.world * n, self.local_hq, self.dim), device=result.device, dtype=result.dtype)
+        torch.distributed.all_gather_into_tensor(gathered, result.contiguous(), group=self.group)
+        return gathered.view(self.world, n, self.local_hq, self.dim).permute(1, 0, 2, 3)
+
     def _next_positions(self, count):
         positions = [self.prefix_size + r * self.max_new_tokens + self.generated for r in range(count)]
         self.generated += 1
@@ -207,42 +338,30 @@ class SharedKVDecoder:
         self.used += len(token_ids)
         return positions
 
-    def _attention_forward(self, prepared, targets, nreq, tails=None):
+    def _attention_forward(self, prepared, positions, targets, nreq, tails=None):
         """The decode-step attention of every layer: q/k/v projections (this rank's heads), q/k RMSNorm,
-        RoPE, append of the new K/V at ``targets`` (a device tensor of pool positions) by one fused launch,
-        tree attention through ``attention_matrix`` and, when sharded, an all-gather of the heads before
+        RoPE, append of the new K/V at ``targets`` (a device tensor of pool positions) by one fused launch
+        (or norm, RoPE and append by one, ``rotary="fused"``), tree attention through ``attention_matrix`` and, when sharded, an all-gather of the heads before
         ``o_proj``.  ``tails = (cached_plan, count, offset)`` lets the first layer's append also set the
         plan's tail lengths to ``count + offset`` on the device."""
-        pools, slices, decoder = self.pools, self._slices, self
+        pools, decoder = self.pools, self
 
         def forward(module, hidden_states, position_embeddings, attention_mask=None, **kwargs):
             shape = (*hidden_states.shape[:-1], -1, module.head_dim)
-            if slices is None:
-                q = module.q_proj(hidden_states)
-                k = module.k_proj(hidden_states)
-                v = module.v_proj(hidden_states)
-            else:
-                qs, ks = slices
-                q = torch.nn.functional.linear(hidden_states, module.q_proj.weight[qs],
-                                               None if module.q_proj.bias is None else module.q_proj.bias[qs])
-                k = torch.nn.functional.linear(hidden_states, module.k_proj.weight[ks],
-                                               None if module.k_proj.bias is None else module.k_proj.bias[ks])
-                v = torch.nn.functional.linear(hidden_states, module.v_proj.weight[ks],
-                                               None if module.v_proj.bias is None else module.v_proj.bias[ks])
-            q = module.q_norm(q.view(shape)).transpose(1, 2)
-            k = module.k_norm(k.view(shape)).transpose(1, 2)
-            v = v.view(shape).transpose(1, 2)
-            q, k = _rope(q, k, *position_embeddings)
+            q, k, v = (x.view(shape) for x in decoder._project(module, hidden_states))
             kp, vp = pools[module.layer_idx]
-            append_kv(kp, vp, k[:, :, 0, :], v[:, :, 0, :], targets, prepared.status,
-                      tails if module.layer_idx == 0 else None)
-            result = attention_matrix(q[:, :, 0, :].contiguous(), kp, vp, prepared)
-            if decoder.world > 1:
-                # rank-major concatenation along dim 0 (the form every backend accepts)
-                gathered = torch.empty((decoder.world * nreq, decoder.local_hq, decoder.dim), device=result.device,
-                                       dtype=result.dtype)
-                torch.distributed.all_gather_into_tensor(gathered, result.contiguous(), group=decoder.group)
-                result = gathered.view(decoder.world, nreq, decoder.local_hq, decoder.dim).permute(1, 0, 2, 3)
+            tails_here = tails if module.layer_idx == 0 else None
+            if decoder.rotary == "fused":
+                q = decoder._rotary(module, q[:, 0], k[:, 0], v[:, 0], positions.view(-1), targets, prepared.status,
+                                    tails_here)
+            else:
+                q = module.q_norm(q).transpose(1, 2)
+                k = module.k_norm(k).transpose(1, 2)
+                v = v.transpose(1, 2)
+                q, k = _rope(q, k, *position_embeddings)
+                append_kv(kp, vp, k[:, :, 0, :], v[:, :, 0, :], targets, prepared.status, tails_here)
+                q = q[:, :, 0, :].contiguous()
+            result = decoder._gather(attention_matrix(q, kp, vp, prepared), nreq)
             return module.o_proj(result.reshape(nreq, 1, -1)), None
 
         return forward
@@ -256,7 +375,7 @@ class SharedKVDecoder:
         positions = torch.tensor([[len(s)] for s in self.sequences], device=self.device)
         targets = torch.tensor(self._append(token_ids), device=self.device)
         prepared = self._prepare_plan()
-        forward = self._attention_forward(prepared, targets, len(token_ids))
+        forward = self._attention_forward(prepared, positions, targets, len(token_ids))
         for layer in self.model.model.layers:
             layer.self_attn.forward = MethodType(forward, layer.self_attn)
         try:
@@ -268,13 +387,64 @@ class SharedKVDecoder:
                 layer.self_attn.forward = original
         return self.logits
 
+    # -- beam search --------------------------------------------------------------
+    @torch.inference_mode()
+    def beam_search(self, steps, beams=None, end_token=None):
+        """The ``beams`` best continuations of ``steps`` tokens of every prompt, best first.
+
+        Returns ``(tokens [NREQ, beams, steps] int64, scores [NREQ, beams]
+        float32)``, scores being sums of log-probabilities.  A beam that takes
+        ``end_token`` is finished: it repeats that token and keeps its score.
+        Every step's K/V rows of every beam get their own pool positions, and a
+        beam is a list of positions: the prompts are held once, no K/V row moves
+        when beams are exchanged.  ``beams`` defaults to the constructor's, which
+        bounds it; starts from the prompts (before any ``step``) and leaves the
+        decoder's own state as it was.
+        """
+        beams = self.beams if beams is None else beams
+        if not 1 <= beams <= self.beams:
+            raise ValueError(f"the pools have room for {self.beams} beams")
+        if self.generated:
+            raise ValueError("beam search starts from the prompts")
+        if not 0 < steps <= self.max_new_tokens:
+            raise ValueError("Decode exceeds allocated max_new_tokens")
+        r, dev = len(self.sequences), self.device
+        rows = r * beams
+        # positions and tokens of the beams, moved together when beams are exchanged
+        state = torch.zeros((r, beams, 2, steps), device=dev, dtype=torch.int32)
+        prompts, lens = path_table([self.tree.paths[i] for i in range(r)], dev)
+        table = torch.nn.functional.pad(prompts, (0, steps), value=-1).repeat_interleave(beams, 0)
+        new = (lens.long()[:, None] + torch.arange(steps, device=dev)).repeat_interleave(beams, 0)
+        lens = lens.repeat_interleave(beams)
+        cu = torch.arange(rows + 1, device=dev, dtype=torch.int32)
+        slot = torch.arange(rows, device=dev)
+        end = -1 if end_token is None else end_token
+        scores, _, tokens = beam_select(self.logits[:, None], torch.zeros((r, 1), device=dev), beams)
+        finished = None if end_token is None else tokens == end
+        for t in range(steps):
+            if t:
+                scores, parents, tokens = beam_select(logits.view(r, beams, -1), scores, beams, finished=finished,
+                                                      end_token=end)
+                state = beam_reorder(state, parents)
+                if finished is not None:
+                    finished = finished.gather(1, parents) | (tokens == end)
+            targets = self.prefix_size + t * rows + slot
+            state[:, :, 0, t] = targets.view(r, beams)
+            state[:, :, 1, t] = tokens
+            if t + 1 < steps:
+                table.scatter_(1, new, state[:, :, 0].reshape(rows, steps))
+                hidden = self._run_rows(tokens.view(-1), (lens + t).long(), targets, table, lens + t + 1, cu)
+                logits = self.model.lm_head(hidden)
+        return state[:, :, 1].long(), scores
+
 
 class CachedPrefixDecoder(SharedKVDecoder):
     """Reuse the prompt schedule; only the tails' lengths change per step (reference qwen.py:106-124)."""
 
     def __init__(self, model, sequences, max_new_tokens=32, method="cube", cost_model=None, prefill="shared",
-                 shard=None):
-        super().__init__(model, sequences, max_new_tokens, method, cost_model, prefill, shard)
+                 shard=None, rotary="model", beams=1, chunk_tokens=8192):
+        super().__init__(model, sequences, max_new_tokens, method, cost_model, prefill, shard, rotary, beams,
+                         chunk_tokens)
         prefix = schedule(self.tree, self.hq, self.hk, self.dim, self.method, self.cost_model)
         q = torch.empty((len(self.sequences), self.local_hq, self.dim), device=self.device, dtype=model.dtype)
         self.cached_plan = CachedDecodePlan(prefix, q, self.prefix_size, max_new_tokens, self.local_hk)
@@ -320,7 +490,8 @@ class CachedPrefixDecoder(SharedKVDecoder):
         positions = torch.empty((nreq, 1), dtype=torch.int64, device=dev)
         targets = torch.empty(nreq, dtype=torch.int64, device=dev)
         # the first layer's fused append sets the tails' lengths to t + 1
-        forward = self._attention_forward(self.cached_plan.prepared, targets, nreq, (self.cached_plan, t, 1))
+        forward = self._attention_forward(self.cached_plan.prepared, positions, targets, nreq,
+                                          (self.cached_plan, t, 1))
 
         def body():
             positions.copy_((start_pos + (t - t0))[:, None])
