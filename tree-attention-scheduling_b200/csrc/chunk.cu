@@ -137,6 +137,49 @@ __device__ __forceinline__ void load_tile(uint32_t slot, const uint16_t* pool, c
   __syncwarp();
 }
 
+// The warp's 32 query rows into a tile, 16 bytes of a row per lane and copy
+// (`row` is the lane's own row, `rows` how many of the 32 there are).  Read a
+// row per thread instead, the loads of 32 lines an instruction took 8000 cycles.
+template <int D>
+__device__ __forceinline__ void load_queries(uint32_t tile, int first, const uint16_t* row, int rows, int lane) {
+  constexpr int LPR = D / 8, RPI = 32 / LPR;
+  const int c = lane % LPR, r = lane / LPR;
+  constexpr int kBatch = 32 / RPI < 8 ? 32 / RPI : 8;
+#pragma unroll 1
+  for (int i0 = 0; i0 < rows; i0 += kBatch * RPI) {
+    const uint16_t* from[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      from[i] = reinterpret_cast<const uint16_t*>(
+          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), i0 + i * RPI + r));
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (i0 + i * RPI + r < rows)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tile + swz<D>(first + i0 + i * RPI + r, c)),
+                     "l"(from[i] + c * 8));
+  }
+  cp_async_wait_all();
+}
+
+// Staged rows out to global memory, coalesced: CHUNKS 16-byte chunks of each of
+// the warp's rows, `row` the lane's own destination (null: nothing).
+template <int CHUNKS>
+__device__ __forceinline__ uint32_t staged(int r, int c) {
+  return uint32_t(r * CHUNKS + (c ^ (r & (CHUNKS < 8 ? CHUNKS - 1 : 7)))) * 16u;
+}
+template <int CHUNKS>
+__device__ __forceinline__ void store_rows(const unsigned char* stage, void* row, int lane) {
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    const int r = i * (32 / CHUNKS) + lane / CHUNKS, c = lane % CHUNKS;
+    const unsigned long long to = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), r);
+    const uint4 v = *reinterpret_cast<const uint4*>(stage + staged<CHUNKS>(r, c));
+    if (to) *reinterpret_cast<uint4*>(to + c * 16) = v;
+  }
+  __syncwarp();
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     chunk_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ ChunkMaps maps) {
@@ -348,15 +391,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int limit = mine ? min(w.keys, w.shift + local / G + 1) - w.key0 - (two ? 0 : t * kKeys) : 0;
 
       if (ntiles > 0 && (two || t == 0)) {                    // the row's query, K-major with the swizzle
-        unsigned char* qs = smem + S::off_q + (two ? t : 0) * S::kSlot;
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + int64_t(token) * p.q_st + int64_t(hq) * p.q_sh);
-        if (mine) {
-          uint4 x[D / 8];
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) x[c] = src[c];
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(qs + swz<D>(row, c)) = x[c];
-        }
+        load_queries<D>(smem_u32(smem + S::off_q + (two ? t : 0) * S::kSlot), quad * 32,
+                        p.q + int64_t(token) * p.q_st + int64_t(hq) * p.q_sh, min(32, w.rows - (trow - lane)), lane);
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[Q_FULL + (two ? t : 0)]);
@@ -460,6 +496,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       scale_b *= inv;
       const int64_t index = int64_t(token) * p.hq + hq;
       const float lse = z > 0.f ? (m + fast_log2(z)) * kLn2 : -INFINITY;
+      // rows leave through the tile's query slot, which no MMA reads any more
+      constexpr int kRoom = S::kSlot / kRows;                 // staged bytes of a row
+      unsigned char* stage = smem + S::off_q + (two ? t : 0) * S::kSlot + quad * 32 * kRoom;
+      uint16_t* dst = mine ? p.out + index * D : nullptr;
+      float* part = mine && z > 0.f ? p.part + (int64_t(split) * p.num_tokens * p.hq + index) * D : nullptr;   // (no weight in the merge: not read)
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -476,20 +517,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) y[i] += scale_b > 0.f ? __uint_as_float(o[i]) * scale_b : 0.f;
         }
-        if (!mine) continue;
-        if (p.splits > 1) {
-          if (!(z > 0.f)) continue;                           // no weight in the merge: not read
-          float* dst = p.part + (int64_t(split) * p.num_tokens * p.hq + index) * D + c * 32;
+        if (p.splits > 1) {                                   // f32, kRoom bytes of a row at a time
+          constexpr int kChunks = kRoom / 16, kPer = kRoom / 128;
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(dst + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float4*>(stage + staged<kChunks>(lane, c % kPer * 8 + i)) =
+                make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+          if (c % kPer == kPer - 1)
+            store_rows<kChunks>(stage, part ? part + (c / kPer) * (kRoom / 4) : nullptr, lane);
         } else {
-          uint16_t* dst = p.out + index * D + c * 32;
+          constexpr int kChunks = D / 8;
 #pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            *reinterpret_cast<uint4*>(dst + i) =
-                make_uint4(Elem<T>::pack2(y[i], y[i + 1]), Elem<T>::pack2(y[i + 2], y[i + 3]),
-                           Elem<T>::pack2(y[i + 4], y[i + 5]), Elem<T>::pack2(y[i + 6], y[i + 7]));
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(stage + staged<kChunks>(lane, 4 * c + i)) =
+                make_uint4(Elem<T>::pack2(y[8 * i], y[8 * i + 1]), Elem<T>::pack2(y[8 * i + 2], y[8 * i + 3]),
+                           Elem<T>::pack2(y[8 * i + 4], y[8 * i + 5]), Elem<T>::pack2(y[8 * i + 6], y[8 * i + 7]));
+          if (c == D / 32 - 1) store_rows<kChunks>(stage, dst, lane);
         }
       }
       if (mine) {
