@@ -170,12 +170,21 @@ __device__ __forceinline__ uint32_t staged(int r, int c) {
 template <int CHUNKS>
 __device__ __forceinline__ void store_rows(const unsigned char* stage, void* row, int lane) {
   __syncwarp();
+  constexpr int kBatch = CHUNKS < 8 ? CHUNKS : 8;
+  const int c = lane % CHUNKS, r0 = lane / CHUNKS;
 #pragma unroll
-  for (int i = 0; i < CHUNKS; ++i) {
-    const int r = i * (32 / CHUNKS) + lane / CHUNKS, c = lane % CHUNKS;
-    const unsigned long long to = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), r);
-    const uint4 v = *reinterpret_cast<const uint4*>(stage + staged<CHUNKS>(r, c));
-    if (to) *reinterpret_cast<uint4*>(to + c * 16) = v;
+  for (int i0 = 0; i0 < CHUNKS; i0 += kBatch) {
+    uint4 v[kBatch];
+    unsigned long long to[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int r = (i0 + i) * (32 / CHUNKS) + r0;
+      v[i] = *reinterpret_cast<const uint4*>(stage + staged<CHUNKS>(r, c));
+      to[i] = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), r);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (to[i]) *reinterpret_cast<uint4*>(to[i] + c * 16) = v[i];
   }
   __syncwarp();
 }
@@ -501,21 +510,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       unsigned char* stage = smem + S::off_q + (two ? t : 0) * S::kSlot + quad * 32 * kRoom;
       uint16_t* dst = mine ? p.out + index * D : nullptr;
       float* part = mine && z > 0.f ? p.part + (int64_t(split) * p.num_tokens * p.hq + index) * D : nullptr;   // (no weight in the merge: not read)
+      uint32_t o[D / 32][32];                                 // the whole row: loads in flight, one wait
+      if (ntiles > 0) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) tmem_ld32(lane_addr + kColO + (two ? t * 128 : 0) + c * 32, o[c]);
+        tmem_wait_ld();
+      }
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
         float y[32];
-        if (ntiles > 0) {
-          tmem_ld32(lane_addr + kColO + (two ? t * 128 : 0) + c * 32, o);
-          tmem_wait_ld();
-        }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) y[i] = scale_a > 0.f ? __uint_as_float(o[i]) * scale_a : 0.f;
+        for (int i = 0; i < 32; ++i) y[i] = scale_a > 0.f ? __uint_as_float(o[c][i]) * scale_a : 0.f;
         if (joined) {
-          tmem_ld32(lane_addr + kColO + 128 + c * 32, o);
+          uint32_t other[32];
+          tmem_ld32(lane_addr + kColO + 128 + c * 32, other);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) y[i] += scale_b > 0.f ? __uint_as_float(o[i]) * scale_b : 0.f;
+          for (int i = 0; i < 32; ++i) y[i] += scale_b > 0.f ? __uint_as_float(other[i]) * scale_b : 0.f;
         }
         if (p.splits > 1) {                                   // f32, kRoom bytes of a row at a time
           constexpr int kChunks = kRoom / 16, kPer = kRoom / 128;
@@ -644,7 +655,7 @@ Plan choose_plan(int64_t tokens, int64_t seqs, int64_t group, int64_t hk, int64_
   const int64_t rows = plan.small ? kSmallRows : kPairRows;
   plan.tiles = tokens * group / rows + std::min(tokens, seqs);
   const int64_t step = plan.small ? kSmallKeys : kKeys, slots = plan.small ? kSmallCtas * sms : sms;
-  const int64_t kFixed = plan.small ? 30 : 45, kPerStep = plan.small ? 12 : 10, kMerge = 25;
+  const int64_t kFixed = plan.small ? 30 : 75, kPerStep = plan.small ? 12 : 19, kMerge = 25;
   const int64_t base = plan.tiles * hk, steps = std::max<int64_t>(1, (most_keys + step - 1) / step);
   int64_t least = INT64_MAX;
   for (int64_t s = 1; s <= std::min<int64_t>(kMaxSplits, steps); ++s) {
