@@ -642,20 +642,21 @@ struct Plan {
   int64_t tiles;       // row tiles that the batch can have at most
   int splits;
   int split_keys;
+  bool cluster;        // the splits join by themselves (no workspace, no merge)
 };
 
 // Batches of at most kSmallRows rows a sequence on average run on the small-row
 // kernel, others on the tensor-core tiles.  The keys are cut where that lowers
 // a modelled time (tenths of a microsecond; measured on one B200): the waves of
 // CTAs, each kFixed plus kPerStep a step of keys, and the merge of the splits,
-// kMerge plus its bytes at 3 TB/s.
+// kMerge plus its bytes at 3 TB/s, or kJoin within a cluster.
 Plan choose_plan(int64_t tokens, int64_t seqs, int64_t group, int64_t hk, int64_t dim, int64_t most_keys, int sms) {
   Plan plan{};
   plan.small = tokens * group <= kSmallRows * seqs;
   const int64_t rows = plan.small ? kSmallRows : kPairRows;
   plan.tiles = tokens * group / rows + std::min(tokens, seqs);
   const int64_t step = plan.small ? kSmallKeys : kKeys, slots = plan.small ? kSmallCtas * sms : sms;
-  const int64_t kFixed = plan.small ? 30 : 75, kPerStep = plan.small ? 12 : 19, kMerge = 25;
+  const int64_t kFixed = plan.small ? 30 : 75, kPerStep = plan.small ? 12 : 19, kMerge = 25, kJoin = 8;
   const int64_t base = plan.tiles * hk, steps = std::max<int64_t>(1, (most_keys + step - 1) / step);
   int64_t least = INT64_MAX;
   for (int64_t s = 1; s <= std::min<int64_t>(kMaxSplits, steps); ++s) {
@@ -663,19 +664,21 @@ Plan choose_plan(int64_t tokens, int64_t seqs, int64_t group, int64_t hk, int64_
     if (s > 1 && (steps + per - 1) / per != s) continue;     // the same cut as a smaller s
     const int64_t waves = (base * s + slots - 1) / slots;
     int64_t cost = waves * (kFixed + per * kPerStep);
-    if (s > 1) cost += kMerge + s * tokens * group * hk * (dim + 1) * 8 / 300000;
+    const bool cluster = plan.small && s > 1 && s <= kMaxCluster && waves == 1;
+    if (s > 1) cost += cluster ? kJoin : kMerge + s * tokens * group * hk * (dim + 1) * 8 / 300000;
     if (cost < least) {
       least = cost;
       plan.splits = int(s);
       plan.split_keys = int(std::min<int64_t>(per * step, INT32_MAX));
+      plan.cluster = cluster;
     }
     if (s > 1 && waves > 16) break;
   }
   return plan;
 }
 
-int64_t partial_bytes(int splits, int64_t tokens, int64_t hq, int64_t dim) {
-  return splits > 1 ? int64_t(splits) * tokens * hq * (dim + 1) * 4 : 0;
+int64_t partial_bytes(const Plan& plan, int64_t tokens, int64_t hq, int64_t dim) {
+  return plan.splits > 1 && !plan.cluster ? int64_t(plan.splits) * tokens * hq * (dim + 1) * 4 : 0;
 }
 
 // A pool [heads, tokens, D] as boxes of 64 columns x `rows` tokens, 128-byte swizzle.
@@ -745,7 +748,7 @@ extern "C" int64_t ta_chunk_workspace_bytes(int32_t num_tokens, int32_t num_seqs
     return 0;
   const Plan plan = choose_plan(num_tokens, num_seqs, num_q_heads / num_kv_heads, num_kv_heads, head_dim,
                                 int64_t(table_width) * page_size, sm_count());
-  return partial_bytes(plan.splits, num_tokens, num_q_heads, head_dim);
+  return partial_bytes(plan, num_tokens, num_q_heads, head_dim);
 }
 
 extern "C" int ta_chunk_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* kpool,
@@ -775,7 +778,7 @@ extern "C" int ta_chunk_attention(const void* q, int64_t q_stride_token, int64_t
   if (!aligned(q) || !aligned(kpool) || !aligned(vpool) || !aligned(out) || q_stride_token < 0 || q_stride_head < 0 ||
       (q_stride_token & 7) || (q_stride_head & 7))
     return TA_ERR_ARG;
-  const int64_t need = partial_bytes(plan.splits, num_tokens, num_q_heads, head_dim);
+  const int64_t need = partial_bytes(plan, num_tokens, num_q_heads, head_dim);
   if (need > 0 && (!workspace || !aligned(workspace))) return TA_ERR_ARG;
   if (workspace_bytes < need) return TA_ERR_TOO_LARGE;
   ChunkParams p{};
@@ -791,7 +794,7 @@ extern "C" int ta_chunk_attention(const void* q, int64_t q_stride_token, int64_t
   p.hq = num_q_heads, p.hk = num_kv_heads, p.group = group;
   p.causal = causal != 0;
   p.out = static_cast<uint16_t*>(out), p.lse = out_lse;
-  p.splits = plan.splits, p.split_keys = plan.split_keys;
+  p.splits = plan.splits, p.split_keys = plan.split_keys, p.cluster = plan.cluster;
   p.part = static_cast<float*>(workspace);
   p.part_lse = p.part + int64_t(plan.splits) * num_tokens * num_q_heads * head_dim;
   p.status = status;
@@ -803,7 +806,7 @@ extern "C" int ta_chunk_attention(const void* q, int64_t q_stride_token, int64_t
   else
     err = dtype == TA_DTYPE_BF16 ? launch_dim<__nv_bfloat16>(p, plan.tiles, head_dim, st)
                                  : launch_dim<__half>(p, plan.tiles, head_dim, st);
-  if (err == cudaSuccess && plan.splits > 1)
+  if (err == cudaSuccess && plan.splits > 1 && !plan.cluster)
     err = dtype == TA_DTYPE_BF16 ? launch_chunk_merge<__nv_bfloat16>(p, head_dim, st)
                                  : launch_chunk_merge<__half>(p, head_dim, st);
   return err == cudaSuccess ? TA_OK : TA_ERR_LAUNCH;

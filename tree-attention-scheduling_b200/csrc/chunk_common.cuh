@@ -21,6 +21,7 @@ struct ChunkParams {
   float scale_log2;
   int32_t width, page_shift, num_seqs, num_tokens, hq, hk, group, causal, splits, split_keys;
   int32_t box_rows;                        // rows of the TMA boxes (0: no box maps)
+  int32_t cluster;                         // the splits of a row tile are a cluster and join by themselves
 };
 
 // What a CTA works on: up to ROWS query rows of a sequence and KV head over a range of keys.
@@ -117,6 +118,8 @@ __device__ __forceinline__ Work find_work(const ChunkParams& p, int block, int s
 constexpr int kSmallRows = 16;
 // Resident CTAs an SM of the small-row kernel, and the keys its splits are multiples of.
 constexpr int kSmallCtas = 2, kSmallKeys = 64;
+// Its splits that can join in a cluster (the portable size).
+constexpr int kMaxCluster = 8;
 
 cudaError_t launch_chunk_rows(const ChunkParams& p, int64_t tiles, int head_dim, int dtype, cudaStream_t stream);
 
