@@ -48,6 +48,50 @@ __device__ __forceinline__ Work find_work(const ChunkParams& p, int block, int s
   w.seq = -1, w.rows = 0, w.count = 0;
   w.head = block % p.hk;
   const int tile = block / p.hk;
+  // row tile `local` (from the last) of the `tiles` of a sequence of n tokens from `first` on
+  auto resolve = [&](int seq, int first, int n, int keys, int tiles, int local) {
+    w.seq = seq;
+    w.token0 = first;
+    w.row0 = (tiles - 1 - local) * ROWS;
+    w.rows = min(ROWS, n * p.group - w.row0);
+    const int64_t most = int64_t(p.width) << p.page_shift;
+    if (keys < 0 || keys > most) {
+      set_status(p.status, TA_ERR_BOUNDS);
+      keys = keys < 0 ? 0 : int(most);
+    }
+    w.keys = keys;
+    w.shift = p.causal ? keys - n : INT32_MAX / 2;
+    // keys that the CTA's last row sees
+    const int seen = max(0, min(keys, w.shift + (w.row0 + w.rows - 1) / p.group + 1));
+    const int64_t start = int64_t(split) * p.split_keys;
+    w.key0 = int(min(start, int64_t(seen)));
+    w.count = int(min(start + int64_t(p.split_keys), int64_t(seen))) - w.key0;
+  };
+
+  if (p.num_seqs <= 32) {                   // a sequence a lane: the longest contexts first
+    const int first = p.cu[min(lane, p.num_seqs)], last = p.cu[min(lane + 1, p.num_seqs)];
+    const int keys = p.lens[min(lane, p.num_seqs - 1)];
+    int n = last - first;                   // 0 past the last sequence
+    if (first < 0 || last < first || last > p.num_tokens) {
+      set_status(p.status, TA_ERR_BOUNDS);
+      n = 0;
+    }
+    const int tiles = int((int64_t(n) * p.group + ROWS - 1) / ROWS);
+    int before = 0;
+    for (int j = 0; j < p.num_seqs; ++j) {
+      const int theirs = __shfl_sync(0xffffffffu, keys, j), count = __shfl_sync(0xffffffffu, tiles, j);
+      before += theirs > keys || (theirs == keys && j < lane) ? count : 0;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, lane < p.num_seqs && tile >= before && tile < before + tiles);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      resolve(src, __shfl_sync(0xffffffffu, first, src), __shfl_sync(0xffffffffu, n, src),
+              __shfl_sync(0xffffffffu, keys, src), __shfl_sync(0xffffffffu, tiles, src),
+              tile - __shfl_sync(0xffffffffu, before, src));
+    }
+    return w;
+  }
+
   int before = 0;
   for (int b0 = 0; b0 < p.num_seqs; b0 += 32 * kSeqs) {
     int edge[kSeqs + 1], len[kSeqs];
@@ -87,26 +131,9 @@ __device__ __forceinline__ Work find_work(const ChunkParams& p, int block, int s
           local -= from;
         }
       }
-      local = __shfl_sync(0xffffffffu, local, src);
-      tiles = __shfl_sync(0xffffffffu, tiles, src);
-      n = __shfl_sync(0xffffffffu, n, src);
-      keys = __shfl_sync(0xffffffffu, keys, src);
-      w.seq = __shfl_sync(0xffffffffu, seq, src);
-      w.token0 = __shfl_sync(0xffffffffu, first, src);
-      w.row0 = (tiles - 1 - local) * ROWS;
-      w.rows = min(ROWS, n * p.group - w.row0);
-      const int64_t most = int64_t(p.width) << p.page_shift;
-      if (keys < 0 || keys > most) {
-        set_status(p.status, TA_ERR_BOUNDS);
-        keys = keys < 0 ? 0 : int(most);
-      }
-      w.keys = keys;
-      w.shift = p.causal ? keys - n : INT32_MAX / 2;
-      // keys that the CTA's last row sees
-      const int seen = max(0, min(keys, w.shift + (w.row0 + w.rows - 1) / p.group + 1));
-      const int64_t start = int64_t(split) * p.split_keys;
-      w.key0 = int(min(start, int64_t(seen)));
-      w.count = int(min(start + int64_t(p.split_keys), int64_t(seen))) - w.key0;
+      resolve(__shfl_sync(0xffffffffu, seq, src), __shfl_sync(0xffffffffu, first, src),
+              __shfl_sync(0xffffffffu, n, src), __shfl_sync(0xffffffffu, keys, src),
+              __shfl_sync(0xffffffffu, tiles, src), __shfl_sync(0xffffffffu, local, src));
       return w;
     }
     before += __shfl_sync(0xffffffffu, all, 31);
