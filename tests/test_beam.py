@@ -159,6 +159,15 @@ def test_masks_dead_and_finished_beams(dtype):
 
 
 @pytest.mark.gpu
+def test_many_requests_and_equal_beams():
+    """More requests than CTAs, and every candidate equal: the exact bound of the merge."""
+    g = torch.Generator().manual_seed(12)
+    check(torch.randn(700, 3, 50, generator=g).cuda(), -torch.rand(700, 3, generator=g).cuda(), 6)
+    check(torch.zeros(1, 32, 30000, device="cuda"), torch.zeros(1, 32, device="cuda"), 32)
+    check(torch.zeros(1, 32, 100, device="cuda"), torch.zeros(1, 32, device="cuda"), 32)
+
+
+@pytest.mark.gpu
 def test_nan_and_infinite_logits():
     g = torch.Generator().manual_seed(8)
     logits = torch.randn(3, 4, 10000, generator=g)
@@ -167,6 +176,27 @@ def test_nan_and_infinite_logits():
     logits[1, 3, [5, 9999]] = math.inf
     logits[2, 0] = float("nan")
     check(logits.cuda(), -3 * torch.rand(3, 4, generator=g).cuda(), 6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_tokens_masked_with_the_lowest_value(dtype):
+    """Slices and beams wholly at the type's lowest value, and logits at either side of what the sums are scaled by."""
+    t = DTYPES[dtype]
+    g = torch.Generator().manual_seed(13)
+    logits = torch.randn(4, 3, 20000, generator=g).to(t)
+    lowest = torch.finfo(t).min
+    logits[0, :, 5000:] = lowest                             # whole slices
+    logits[1, :, 3:] = lowest                                # fewer tokens than are kept
+    logits[2, 0] = lowest                                    # a whole beam: every token alike
+    logits[2, 1] = lowest / 2
+    logits[2, 1, 700] = lowest / 4
+    logits[3] = -200000.0
+    logits[3, 0, 100] = -131072.0                            # one slice scaled by a power of two, another below it
+    logits[3, 0, 15000] = -131584.0
+    logits[3, 1, 15000] = -199680.0
+    check(logits.cuda(), -3 * torch.rand(4, 3, generator=g).cuda(), 5)
+    check(logits.cuda(), -3 * torch.rand(4, 3, generator=g).cuda(), 32)
 
 
 @pytest.mark.gpu

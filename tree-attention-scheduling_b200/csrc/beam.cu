@@ -49,8 +49,9 @@ struct BeamEntry {     // a listed candidate of a slice
   int32_t token;       // -1: none
 };
 
-// workspace: per (beam row, slice) the sum of exponentials (f64), the maximum
-// (f32) and k entries, as three arrays
+// workspace: per (beam row, slice) the sum of exponentials (f64), the exponent of
+// its unit (f32) and k entries, as three arrays.  The unit is 2^top, or e^top
+// where the sum is negated.
 struct BeamWork {
   double* sum;
   BeamEntry* entries;
@@ -266,13 +267,16 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamParams 
     part = two.f.x + two.f.y;
   }
   // NaN counts as -inf and what is above kMaxLogit as that; both are rare
-  // enough to be found by what they do to the sum and the maximum
-  if (__syncthreads_or(!(part < INFINITY) || top > kMaxLogit)) {
+  // enough to be found by what they do to the sum and the maximum.  A slice
+  // wholly below -kMaxLogit (tokens ruled out by the type's lowest value) has no
+  // whole M that an f32 holds: its sum is in units of e^top.
+  const bool faint = top < -kMaxLogit;                       // (or -inf: its sum is 0 either way)
+  if (__syncthreads_or(!(part < INFINITY) || top > kMaxLogit || faint)) {
     part = 0.f;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
       x[i] = fminf(fmaxf(x[i], -INFINITY), kMaxLogit);
-      if (x[i] > -INFINITY) part += weight(splat(x[i])).f.x;
+      if (x[i] > -INFINITY) part += faint ? fast_exp2((x[i] - top) * kLog2e) : weight(splat(x[i])).f.x;
     }
     bound = -INFINITY;                                     // the exact bound below
   }
@@ -296,7 +300,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_slice_kernel(BeamParams 
     double total = s_warp_sum[tid];
 #pragma unroll
     for (int off = kBeamWarps / 2; off >= 1; off >>= 1) total += __shfl_xor_sync((1u << kBeamWarps) - 1, total, off);
-    if (tid == 0) p.work.sum[out] = total, p.work.top[out] = top > -INFINITY ? M : -INFINITY;
+    if (tid == 0) p.work.sum[out] = faint ? -total : total, p.work.top[out] = faint ? top : M;
   }
   uint64_t key_bound = 1;
   if (n > kMaxCand) {
@@ -366,7 +370,8 @@ constexpr int kDepths = 4;
 
 __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamParams p) {
   __shared__ BeamCand s_cand[kMaxCand];
-  __shared__ double s_base[kMaxK];                           // per beam: score - logsumexp
+  __shared__ double s_base[kMaxK];                           // per beam: score - (logsumexp - s_ref)
+  __shared__ float s_ref[kMaxK];                             // 0, or near the logsumexp of a faint beam
   __shared__ uint32_t s_warp[kDepths][kBeamWarps], s_bound[kDepths];
   __shared__ BeamCand s_exact;
   __shared__ int s_count;
@@ -405,11 +410,13 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamParams p) 
     // a slice's sum is in units of 2^M, its M in work.top
     double sum = 0.;
     float M = -INFINITY;
+    bool faint = false;
     for (int s0 = 0; s0 < p.slices; s0 += 32) {              // two of the lane's slices at a time
       const int s = s0 + sub;
       const bool one = has && s < p.slices, two = has && s + 16 < p.slices;
       const float t1 = one ? p.work.top[at + s] : -INFINITY, t2 = two ? p.work.top[at + s + 16] : -INFINITY;
       const double p1 = one ? p.work.sum[at + s] : 0., p2 = two ? p.work.sum[at + s + 16] : 0.;
+      faint |= p1 < 0. || p2 < 0.;
       float up = fmaxf(M, fmaxf(t1, t2));
 #pragma unroll
       for (int off = 8; off >= 1; off >>= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, off));
@@ -418,16 +425,40 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(BeamParams p) 
     }
 #pragma unroll
     for (int off = 8; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (has && sub == 0)
+    if (__any_sync(0xffffffffu, faint)) {                    // rare: every unit as a power of e, in f64
+      auto unit = [&](int s) { return double(p.work.top[at + s]) * (p.work.sum[at + s] < 0. ? 1. : 0.69314718055994530942); };
+      double up = -INFINITY;
+      for (int s = sub; has && s < p.slices; s += 16) up = fmax(up, unit(s));
+#pragma unroll
+      for (int off = 8; off >= 1; off >>= 1) up = fmax(up, __shfl_xor_sync(0xffffffffu, up, off));
+      sum = 0.;
+      for (int s = sub; has && s < p.slices; s += 16) {
+        const double u = unit(s);
+        if (u > -INFINITY) sum += fabs(p.work.sum[at + s]) * exp(u - up);
+      }
+#pragma unroll
+      for (int off = 8; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      // (logits of 1e38 would absorb the score: they are taken less their maximum first)
+      const float ref = up > -INFINITY ? float(up) : 0.f;
+      if (has && sub == 0) {
+        s_ref[w] = ref;
+        s_base[w] = up > -INFINITY ? double(score_of[i]) - ((up - double(ref)) + log(sum)) : -INFINITY;
+      }
+      continue;
+    }
+    if (has && sub == 0) {
+      s_ref[w] = 0.f;
       s_base[w] = M > -INFINITY ? double(score_of[i]) - (double(M) + log2(sum)) * 0.69314718055994530942 : -INFINITY;
+    }
   }
   __syncthreads();
-  auto score = [&](int w, float x) { return x > -INFINITY ? double(x) + s_base[w] : -INFINITY; };
+  auto score = [&](int w, float x) { return x > -INFINITY ? double(x) - double(s_ref[w]) + s_base[w] : -INFINITY; };
   // The same in f32 (f64 is slow here), less or more a margin for its rounding:
   // the bound is taken from lower values, candidates pass by their upper ones.
   auto rough = [&](int w, float x, float side) {
     const float c = float(s_base[w]);
-    return x > -INFINITY && c > -INFINITY ? x + c + side * 4e-7f * (fabsf(x) + fabsf(c)) : -INFINITY;
+    const float y = x - s_ref[w];
+    return x > -INFINITY && c > -INFINITY ? y + c + side * 4e-7f * (fabsf(y) + fabsf(c)) : -INFINITY;
   };
   // beam of a list (exact: lists stay far below 2^20)
   const float per_slice = 1.f / float(p.slices);
