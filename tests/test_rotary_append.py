@@ -206,3 +206,14 @@ def test_refusals_on_gpu():
                    dict(out=x["kp"].flatten()[:4 * 4 * 64].view(4, 4, 64)), dict(status=torch.zeros(1).cuda())):
         with pytest.raises(ValueError):
             rotary_append(**{**x, **change})
+
+
+@pytest.mark.gpu
+def test_inputs_in_the_pools_are_refused():
+    """Rows that lie in the pools would be read and written at once."""
+    from tree_attention.rotary import rotary_append
+    x = inputs(4, 4, 2, 64, 64, torch.bfloat16, 6)
+    for change in (dict(k=x["kp"][:, 3:7].transpose(0, 1)), dict(v=x["vp"][:, 3:7].transpose(0, 1)),
+                   dict(q=x["vp"].flatten()[64:64 + 4 * 4 * 64].view(4, 4, 64))):
+        with pytest.raises(ValueError):
+            rotary_append(**{**x, **change})

@@ -162,6 +162,8 @@ PyObject* rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                       "rotary_append: the cached plan's lengths and tail indices must be int32");
   }
   const c10::cuda::CUDAGuard guard(device);
+  for (const at::Tensor* x : {&q, &k, &v})
+    TORCH_CHECK_VALUE(!overlap(*x, kp) && !overlap(*x, vp), "rotary_append: an input overlaps the pools");
   q = rows16(q), k = rows16(k), v = rows16(v);
   positions = packed(positions), targets = packed(targets), freq = packed(freq);
   for (at::Tensor* w : {&qw, &kw})
@@ -237,6 +239,8 @@ PyObject* chunk_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   TORCH_CHECK_VALUE(!lse.defined() || (lse.dim() == 2 && lse.size(0) == n && lse.size(1) == hq &&
                                        lse.scalar_type() == at::kFloat && lse.is_contiguous()),
                     "chunk_attention: out_lse must be contiguous float32 [N, HQ] on q's device");
+  TORCH_CHECK_VALUE(!lse.defined() || !(overlap(lse, out) || overlap(lse, q) || overlap(lse, kp) || overlap(lse, vp)),
+                    "chunk_attention: out_lse overlaps another tensor");
   if (n > 0 && b > 0) {
     const int32_t tokens = narrow(n, "N"), seqs = narrow(b, "B"), heads = narrow(hq, "HQ"), width = narrow(table.size(1), "W"),
                   rows = narrow(page, "page_size");
