@@ -97,6 +97,14 @@ def run(batch, **kwargs):
     return out, lse
 
 
+def run_quietly(batch):
+    """``run`` without a synchronisation."""
+    from tree_attention.chunk import chunk_attention
+    lse = torch.empty(batch["q"].shape[:2], device="cuda")
+    return chunk_attention(batch["q"], batch["kp"], batch["vp"], batch["table"], batch["lens"], batch["cu"],
+                           page_size=batch["page"], out_lse=lse), lse
+
+
 # ---- on the CPU: refusals ------------------------------------------------------
 def test_validation_without_gpu():
     lib = _lib.load()
@@ -166,6 +174,87 @@ def test_ragged_batch(shape, page):
 @pytest.mark.parametrize("shape", [(32, 8, 128), (4, 4, 128), (6, 2, 64), (4, 2, 32)], ids=lambda s: "x".join(map(str, s)))
 def test_chunk(shape, fresh, total, dtype):
     batch = make_batch([fresh], [total], *shape, 1, DTYPES[dtype], fresh)
+    check(batch, *run(batch))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [32, 33, 129, 300])
+@pytest.mark.parametrize("chunk", [1, 40])
+def test_many_sequences(count, chunk):
+    """More sequences than a lane or a round of the block lookup takes, some without tokens or keys."""
+    g = torch.Generator().manual_seed(count)
+    fresh = torch.randint(0, chunk + 1, (count,), generator=g).tolist()
+    total = [n + t for n, t in zip(fresh, torch.randint(0, 200, (count,), generator=g).tolist())]
+    batch = make_batch(fresh, total, 8, 2, 64, 16, torch.bfloat16, count)
+    check(batch, *run(batch))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(32, 1, 128), (71, 1, 64), (40, 2, 32)], ids=lambda s: "x".join(map(str, s)))
+def test_large_groups(shape):
+    """More GQA rows a token than the small-row kernel takes, and groups that no tile is a multiple of."""
+    for fresh, total in (([1] * 5, [400, 1, 33, 0, 129]), ([9, 70], [300, 70])):
+        batch = make_batch(fresh, total, *shape, 1, torch.float16, 20)
+        check(batch, *run(batch))
+
+
+@pytest.mark.gpu
+def test_uneven_batch_on_the_small_row_kernel():
+    """Few rows a sequence on average, one long chunk among empty sequences: many 16-row tiles of one sequence."""
+    fresh, total = [0] * 60 + [150] + [0] * 39, [5] * 60 + [400] + [0] * 39
+    batch = make_batch(fresh, total, 8, 2, 128, 1, torch.bfloat16, 21)
+    check(batch, *run(batch))
+
+
+@pytest.mark.gpu
+def test_consecutive_positions():
+    """Runs of positions, as the nodes of a tree have: whole tiles, runs that end inside a tile, the pool's end."""
+    for shape in ((8, 2, 128), (8, 2, 64)):
+        batch = make_batch([300, 3], [900, 500], *shape, 1, torch.bfloat16, 22, garbage=False)
+        tokens = batch["kp"].shape[1]
+        paths = [list(range(100, 600)) + list(range(1000, 1300)) + list(range(0, 100)), list(range(tokens - 500, tokens))]
+        batch["paths"] = [torch.tensor(x) for x in paths]
+        for row, path in zip(batch["table"], paths):
+            row[:len(path)] = torch.tensor(path)
+        check(batch, *run(batch))
+        check(batch, *run(batch, causal=False), causal=False)
+
+
+@pytest.mark.gpu
+def test_two_threads_on_their_own_streams():
+    """Calls at once are independent: nothing is shared between them."""
+    from concurrent.futures import ThreadPoolExecutor
+    batches = [make_batch([1] * 4, [900, 20, 333, 1], 8, 2, 128, 1, torch.bfloat16, 23),
+               make_batch([200], [700], 8, 2, 128, 16, torch.bfloat16, 24)]
+    torch.cuda.synchronize()
+
+    def work(batch):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            results = [run_quietly(batch) for _ in range(30)]
+        stream.synchronize()
+        return results
+
+    with ThreadPoolExecutor(2) as pool:
+        for batch, results in zip(batches, pool.map(work, batches)):
+            first = results[0]
+            assert all(torch.equal(a, b) for r in results for a, b in zip(r, first))
+            check(batch, *first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_many_faint_keys(dtype, tokens):
+    """One key 2^19.6 above 600 others and without value: the others' weights are normal numbers of the type."""
+    batch = make_batch([tokens], [600], 4, 2, 64, 1, DTYPES[dtype], 25, garbage=False)
+    batch["q"].zero_()
+    batch["q"][..., 0] = 8.0
+    batch["kp"].zero_()
+    batch["vp"].abs_()
+    first = batch["paths"][0][0]
+    batch["kp"][:, first, 0] = 19.6 * math.log(2)
+    batch["vp"][:, first] = 0
     check(batch, *run(batch))
 
 
@@ -315,3 +404,15 @@ def test_refusals_on_gpu():
         with pytest.raises(ValueError):
             chunk_attention(**{**good, **change})
     assert chunk_attention(**{**good, "q": b["q"][:0], "cu_q": torch.zeros(2, device="cuda").int()}).shape == (0, 8, 64)
+
+
+@pytest.mark.gpu
+def test_overlapping_outputs_are_refused():
+    from tree_attention.chunk import chunk_attention
+    b = make_batch([2], [40], 8, 2, 64, 16, torch.bfloat16, 26)
+    good = dict(q=b["q"], kp=b["kp"], vp=b["vp"], table=b["table"], kv_lens=b["lens"], cu_q=b["cu"], page_size=16)
+    out = torch.empty_like(b["q"])
+    for lse in (out.view(torch.float32).flatten()[-16:].view(2, 8), b["q"].view(torch.float32).flatten()[:16].view(2, 8),
+                b["vp"].view(torch.float32).flatten()[:16].view(2, 8)):
+        with pytest.raises(ValueError):
+            chunk_attention(**good, out=out, out_lse=lse)

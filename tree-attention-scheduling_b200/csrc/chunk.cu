@@ -30,7 +30,8 @@
 // S_t and P_t share TMEM columns; O_t accumulates in TMEM and is rescaled only
 // when a row's maximum grows by more than 2^8 (exact after the division).  P is
 // rounded to the input type for P.V (a relative 2^-9 or 2^-12 per weight, at
-// random); sums and the LSE use the unrounded f32 weights.
+// random; f16 weights below 2^-21 of the maximum 2^-32 of it); sums and the LSE
+// use the unrounded f32 weights.
 //
 // When the (tile, KV head) pairs do not fill the GPU the keys are cut into
 // splits whose normalised f32 partials chunk_merge_kernel combines by LSE.
@@ -444,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         z *= alpha;
         m_run = m_new;
         // a row without a visible key so far: exp2(-inf - 0) = 0
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float m_use = m_new == -INFINITY ? 0.f : m_new - kWeightShift<T>;
         F2 sum = splat(0.f);
         const F2 sc = splat(scale), neg_m = splat(-m_use);
 #pragma unroll
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       scale_a = z > 0.f ? scale_a * inv : 0.f;
       scale_b *= inv;
       const int64_t index = int64_t(token) * p.hq + hq;
-      const float lse = z > 0.f ? (m + fast_log2(z)) * kLn2 : -INFINITY;
+      const float lse = z > 0.f ? (m - kWeightShift<T> + fast_log2(z)) * kLn2 : -INFINITY;
       // rows leave through the tile's query slot, which no MMA reads any more
       constexpr int kRoom = S::kSlot / kRows;                 // staged bytes of a row
       unsigned char* stage = smem + S::off_q + (two ? t : 0) * S::kSlot + quad * 32 * kRoom;

@@ -141,6 +141,11 @@ __device__ __forceinline__ Work find_work(const ChunkParams& p, int block, int s
   return w;
 }
 
+// Softmax weights are carried times 2^kWeightShift: up to 2^8 above the running
+// maximum, they lie in [0, 2^15] in f16, whose normal range then reaches 2^-21 of
+// the maximum (2^-14 unshifted, a long context's faint keys).
+template <typename T> constexpr float kWeightShift = Elem<T>::kCode == TA_DTYPE_F16 ? 7.f : 0.f;
+
 // Rows of at most kSmallRows (token x GQA row) a sequence: chunk_rows.cu.
 constexpr int kSmallRows = 16;
 // Resident CTAs an SM of the small-row kernel, and the keys its splits are multiples of.
