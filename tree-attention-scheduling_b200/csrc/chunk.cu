@@ -37,6 +37,13 @@
 // splits whose normalised f32 partials chunk_merge_kernel combines by LSE.
 // Batches of few rows a sequence (decode steps) run on the kernel of
 // chunk_rows.cu instead, with the same splits and merge.
+//
+// Bound by each stream's chain of products and softmax: 3650 cycles a pair of
+// tiles (D = 128), 2050 of them MMAs and as many ex2; a document of 8128 tokens,
+// 32/8 heads: 489 us, 1.1 PFLOP/s; 6 ragged chunks of up to 391 tokens over up to
+// 3064 keys: 82 us; 5 x 777 tokens over 2300 keys, 16/2 heads of 64: 46 us.  MMAs
+// of 64 keys take as long as those of 128, so smaller steps do not shorten it
+// (654 us with S of 64 keys in two buffers).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
