@@ -12,30 +12,38 @@
 // Angles: t reaches 1e6 rad and more in a long context, where an f32 product
 // is off by 0.06 rad.  t / 2 pi is taken in f64 (a position and an f32
 // frequency multiply exactly), reduced to a fraction of a turn, and only that
-// fraction is rounded to f32 (2^-25 turns) for sincospif.  The rotary_dim / 2
-// sines of a token are computed once per CTA and shared by all its heads.
+// fraction is rounded to f32 (2^-25 turns) for sincospif.
 //
-// Bound: HBM, if the instructions stay few: a thread owns the two 16-byte chunks
-// of a row that hold both elements of eight pairs (so no exchange between
-// lanes), always the same columns and rows: its pointers, weights and, for a
-// token, sines and cosines are set up once.  A CTA walks tokens with up to 64
-// rows (head_dim 128); the next token's sines are computed while the current
-// one's rows are under way, one barrier a token.
+// A thread owns the two 16-byte chunks of a row that hold both elements of eight
+// pairs (so no exchange between lanes), always the same columns: a token's sines
+// and cosines, computed once and shared through shared memory, stay in its
+// registers over the token's rows.  Two forms:
+//
+//   rows    while a CTA a token (and 128 / lanes-a-row rows) fits one wave, where
+//           it is latency that counts: 16 tokens of 32 + 8 + 8 heads of 128 2.9 us
+//   tokens  beyond: a warp walks whole tokens, four rows a lane in flight, no
+//           barrier but __syncwarp; the next batch's or token's loads wait for
+//           nothing.  16384 such tokens: 73 us, 5.5 TB/s read and written.  A CTA
+//           a token with a barrier and three rows a thread: 78 (4096 tokens:
+//           23.4 against 24.8, as 2960 warps share them unevenly).
+//
+// Bound: HBM, if the instructions stay few: packed f32 pairs, issue slots half used.
 #include <algorithm>
 
 #include "ta_common.cuh"
 #include "ta_kernels.cuh"
+#include "tc_common.cuh"
 
 namespace ta {
 
 namespace {
 
 constexpr int kRotaryThreads = 128;
-// Rows of a thread and resident CTAs an SM: three rows for long inputs (16384
-// tokens of 32 + 8 + 8 heads: 78 us; one row 87, four rows 79); one row while
-// the CTAs fit one wave, where it is latency that counts (16 tokens: 2.9 us
-// against 3.8 with three rows).
-template <int R> constexpr int kCtas = R == 1 ? 8 : 5;
+constexpr int kWarps = kRotaryThreads / 32;
+constexpr int kRowsCtas = 8;                    // CTAs of the rows form an SM
+// Rows of a lane in flight and CTAs an SM of the tokens form (16384 tokens: 3 rows
+// 74 us, 6 rows on 4 CTAs 75; 4 rows on 6 CTAs, spilling, 82).
+constexpr int kBatch = 4, kTokenCtas = 5;
 
 struct RotaryParams {
   const uint16_t *q, *k, *v;
@@ -55,157 +63,208 @@ struct RotaryParams {
   int num_tokens, hq, hk, half, interleaved, num_tails, offset, num_jobs;
 };
 
-template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = Elem<T>::to_float2(w[i]);
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
+// The tails' lengths of a captured decode step's first layer, by one CTA.
+__device__ __forceinline__ void set_tails(const RotaryParams& p) {
+  const int64_t value = *p.count + p.offset;
+  for (int i = threadIdx.x; i < p.num_tails; i += kRotaryThreads) {
+    const int j = p.tail_jobs[i];
+    if (j < 0 || j >= p.num_jobs || value < 0 || value > INT32_MAX)
+      set_status(p.status, TA_ERR_BOUNDS);
+    else
+      p.klen[j] = int32_t(value);
   }
 }
 
-template <typename T, int D, bool PAIRS, int R>  // PAIRS: (2i, 2i + 1), else (i, i + rotary_dim / 2); R rows a thread
-__global__ void __launch_bounds__(kRotaryThreads, kCtas<R>) rotary_append_kernel(const __grid_constant__ RotaryParams p) {
-  constexpr int LPR = D / 16;                   // lanes of a row
-  constexpr int RPP = kRotaryThreads / LPR;     // rows of a pass of the CTA
-  __shared__ __align__(16) float s_cos[2][D / 2], s_sin[2][D / 2];
-  const int tid = threadIdx.x;
+// Sines and cosines of a position's pairs i = first, first + step, ..., times the attention factor.
+__device__ __forceinline__ void sines(const RotaryParams& p, int64_t position, int first, int step, float* cosines,
+                                      float* sines) {
+  const double turn = double(position) * 0.15915494309189533577;               // 1 / 2 pi
+  for (int i = first; i < p.half; i += step) {
+    const double t = turn * double(p.inv_freq[i]);
+    float s, c;
+    sincospif(2.f * float(t - rint(t)), &s, &c);
+    cosines[i] = c * p.factor;
+    sines[i] = s * p.factor;
+  }
+}
 
-  if (p.klen && blockIdx.x == 0 && blockIdx.y == 0) {   // a captured decode step's first layer: the tails' lengths
-    const int64_t value = *p.count + p.offset;
-    for (int i = tid; i < p.num_tails; i += kRotaryThreads) {
-      const int j = p.tail_jobs[i];
-      if (j < 0 || j >= p.num_jobs || value < 0 || value > INT32_MAX)
-        set_status(p.status, TA_ERR_BOUNDS);
-      else
-        p.klen[j] = int32_t(value);
+// The pairs of a thread: 8 j .. 8 j + 7, in chunks c0 and c1 of a row.
+template <bool PAIRS>
+struct Columns {
+  int j, c0, c1;
+  bool turns;
+  __device__ __forceinline__ Columns(const RotaryParams& p, int lane_of_row) : j(lane_of_row) {
+    const int hl = p.half / 8;
+    turns = j < hl;
+    c0 = PAIRS ? 2 * j : turns ? j : 2 * j;
+    c1 = PAIRS || !turns ? c0 + 1 : j + hl;
+  }
+  __device__ __forceinline__ void load(const float* cosines, const float* sines, F2 (&co)[4], F2 (&si)[4]) const {
+    if (!turns) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      co[i].f = *reinterpret_cast<const float2*>(cosines + 8 * j + 2 * i);
+      si[i].f = *reinterpret_cast<const float2*>(sines + 8 * j + 2 * i);
     }
   }
-  const int rows = p.hq + 2 * p.hk;
-  int token = blockIdx.x;
-  if (token >= p.num_tokens || rows == 0) return;
+};
 
-  // this thread's pairs 8j .. 8j + 7 and the chunks they lie in
-  const int j = tid % LPR, hl = p.half / 8;
-  const bool turns = j < hl;
-  const int c0 = PAIRS ? 2 * j : turns ? j : 2 * j, c1 = PAIRS || !turns ? c0 + 1 : j + hl;
-  // its rows: q heads, then k, then v
-  const uint16_t* src[R];
-  uint16_t* dst[R];
-  int kind[R];                      // 0 q, 1 k, 2 v, 3 none
-#pragma unroll
-  for (int u = 0; u < R; ++u) {
-    const int row = (blockIdx.y * R + u) * RPP + tid / LPR;
-    if (row < p.hq) {
-      kind[u] = 0;
-      src[u] = p.q + token * p.q_st + int64_t(row) * p.q_sh;
-      dst[u] = p.q_out + int64_t(row) * D;
-    } else if (row < p.hq + p.hk) {
-      kind[u] = 1;
-      src[u] = p.k + token * p.k_st + int64_t(row - p.hq) * p.k_sh;
-      dst[u] = p.kpool + int64_t(row - p.hq) * p.pool_tokens * D;
-    } else if (row < rows) {
-      kind[u] = 2;
-      src[u] = p.v + token * p.v_st + int64_t(row - p.hq - p.hk) * p.v_sh;
-      dst[u] = p.vpool + int64_t(row - p.hq - p.hk) * p.pool_tokens * D;
-    } else {
-      kind[u] = 3;
-      src[u] = nullptr;
-      dst[u] = nullptr;
-    }
-  }
-  auto sines = [&](int tok, int buffer) {
-    const double turn = double(p.positions[tok]) * 0.15915494309189533577;       // 1 / 2 pi
-    for (int i = tid; i < p.half; i += kRotaryThreads) {
-      const double t = turn * double(p.inv_freq[i]);
-      float s, co;
-      sincospif(2.f * float(t - rint(t)), &s, &co);
-      s_cos[buffer][i] = co * p.factor;
-      s_sin[buffer][i] = s * p.factor;
-    }
-  };
+// Row `row` of a token: q heads (kind 0), then k (1), then v (2); 3 past them.
+__device__ __forceinline__ int kind_of(const RotaryParams& p, int row) {
+  return row < p.hq ? 0 : row < p.hq + p.hk ? 1 : row < p.hq + 2 * p.hk ? 2 : 3;
+}
+__device__ __forceinline__ const uint16_t* source(const RotaryParams& p, int kind, int64_t token, int row) {
+  return kind == 0   ? p.q + token * p.q_st + int64_t(row) * p.q_sh
+         : kind == 1 ? p.k + token * p.k_st + int64_t(row - p.hq) * p.k_sh
+                     : p.v + token * p.v_st + int64_t(row - p.hq - p.hk) * p.v_sh;
+}
+template <int D>
+__device__ __forceinline__ uint16_t* destination(const RotaryParams& p, int kind, int64_t token, int64_t target, int row) {
+  return kind == 0   ? p.q_out + (token * p.hq + row) * D
+         : kind == 1 ? p.kpool + (int64_t(row - p.hq) * p.pool_tokens + target) * D
+                     : p.vpool + (int64_t(row - p.hq - p.hk) * p.pool_tokens + target) * D;
+}
+// Whether the token's k and v are stored (-1: padding).
+__device__ __forceinline__ bool stored_at(const RotaryParams& p, int64_t target, bool reports) {
+  const bool stored = target >= 0 && target < p.pool_tokens;
+  if (!stored && target != -1 && reports) set_status(p.status, TA_ERR_BOUNDS);
+  return stored;
+}
 
-  const bool norm = p.q_weight || p.k_weight;
-  sines(token, 0);
-  for (int buffer = 0;; buffer ^= 1) {
-    uint4 raw[R][2];
+// Norm and turn a thread's chunks of a row of `kind`, in place (v and missing rows stay as they are).
+template <typename T, int D, bool PAIRS>
+__device__ __forceinline__ void turn_row(const RotaryParams& p, int kind, int c0, int c1, bool turns, const F2 (&co)[4],
+                                         const F2 (&si)[4], uint4& lo, uint4& hi) {
+  constexpr int LPR = D / 16;
+  if (__any_sync(0xffffffffu, kind < 2)) {
+    F2 a[4], b[4];
+    const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-    for (int u = 0; u < R; ++u) {
-      if (kind[u] == 3) break;                  // rows only end: later ones are none as well
-      raw[u][0] = *reinterpret_cast<const uint4*>(src[u] + c0 * 8);
-      raw[u][1] = *reinterpret_cast<const uint4*>(src[u] + c1 * 8);
-      src[u] += (kind[u] == 0 ? p.q_st : kind[u] == 1 ? p.k_st : p.v_st) * int64_t(gridDim.x);
+    for (int i = 0; i < 4; ++i) a[i].f = Elem<T>::to_float2(wl[i]), b[i].f = Elem<T>::to_float2(wh[i]);
+    const uint16_t* weight = kind == 0 ? p.q_weight : kind == 1 ? p.k_weight : nullptr;
+    if (p.q_weight || p.k_weight) {
+      F2 sum = splat(0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum = ffma2(b[i], b[i], ffma2(a[i], a[i], sum));
+      float total = sum.f.x + sum.f.y;
+#pragma unroll
+      for (int off = LPR / 2; off >= 1; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+      if (weight) {
+        const F2 scale = splat(rsqrtf(total * (1.f / D) + p.eps));
+        const uint4 ga = *reinterpret_cast<const uint4*>(weight + c0 * 8), gb = *reinterpret_cast<const uint4*>(weight + c1 * 8);
+        const uint32_t xa[4] = {ga.x, ga.y, ga.z, ga.w}, xb[4] = {gb.x, gb.y, gb.z, gb.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          F2 g, h;
+          g.f = Elem<T>::to_float2(xa[i]), h.f = Elem<T>::to_float2(xb[i]);
+          a[i] = fmul2(a[i], fmul2(scale, g));
+          b[i] = fmul2(b[i], fmul2(scale, h));
+        }
+      }
     }
-    const int64_t target = p.targets[token];
-    const bool stored = target >= 0 && target < p.pool_tokens;
-    if (!stored && target != -1 && tid == 0) set_status(p.status, TA_ERR_BOUNDS);
-    const int following = token + gridDim.x;
-    __syncthreads();                            // this token's sines are there, the last one's are read
-    float co[8], si[8];
     if (turns) {
+      if constexpr (PAIRS) {
 #pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        *reinterpret_cast<float4*>(co + i) = *reinterpret_cast<const float4*>(&s_cos[buffer][8 * j + i]);
-        *reinterpret_cast<float4*>(si + i) = *reinterpret_cast<const float4*>(&s_sin[buffer][8 * j + i]);
+        for (int i = 0; i < 4; ++i) {
+          // pairs 2i, 2i + 1 of the first chunk are angles i; the second chunk's 4 + i
+          const float2 cs = co[i >> 1].f, ss = si[i >> 1].f, ct = co[2 + (i >> 1)].f, st = si[2 + (i >> 1)].f;
+          const float ca = i & 1 ? cs.y : cs.x, sa = i & 1 ? ss.y : ss.x, cb = i & 1 ? ct.y : ct.x, sb = i & 1 ? st.y : st.x;
+          a[i].f = make_float2(a[i].f.x * ca - a[i].f.y * sa, a[i].f.y * ca + a[i].f.x * sa);
+          b[i].f = make_float2(b[i].f.x * cb - b[i].f.y * sb, b[i].f.y * cb + b[i].f.x * sb);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          F2 ns;
+          ns.f = make_float2(-si[i].f.x, -si[i].f.y);
+          const F2 x = ffma2(a[i], co[i], fmul2(b[i], ns));
+          b[i] = ffma2(b[i], co[i], fmul2(a[i], si[i]));
+          a[i] = x;
+        }
       }
     }
-    if (following < p.num_tokens) sines(following, buffer ^ 1);
+    if (kind < 2) {
+      lo = make_uint4(Elem<T>::pack2(a[0].f.x, a[0].f.y), Elem<T>::pack2(a[1].f.x, a[1].f.y),
+                      Elem<T>::pack2(a[2].f.x, a[2].f.y), Elem<T>::pack2(a[3].f.x, a[3].f.y));
+      hi = make_uint4(Elem<T>::pack2(b[0].f.x, b[0].f.y), Elem<T>::pack2(b[1].f.x, b[1].f.y),
+                      Elem<T>::pack2(b[2].f.x, b[2].f.y), Elem<T>::pack2(b[3].f.x, b[3].f.y));
+    }
+  }
+}
+
+template <typename T, int D, bool PAIRS>          // PAIRS: (2i, 2i + 1), else (i, i + rotary_dim / 2)
+__global__ void __launch_bounds__(kRotaryThreads, kRowsCtas) rotary_rows_kernel(const __grid_constant__ RotaryParams p) {
+  constexpr int LPR = D / 16;                    // lanes of a row
+  constexpr int kRows = kRotaryThreads / LPR;    // rows of the CTA
+  __shared__ __align__(16) float s_cos[D / 2], s_sin[D / 2];
+  const int tid = threadIdx.x;
+  if (p.klen && blockIdx.x == 0 && blockIdx.y == 0) set_tails(p);
+  const int token = blockIdx.x, row = blockIdx.y * kRows + tid / LPR;
+  if (token >= p.num_tokens) return;
+  const Columns<PAIRS> at(p, tid % LPR);
+  const int kind = kind_of(p, row);
+  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+  if (kind < 3) {
+    const uint16_t* src = source(p, kind, token, row);
+    lo = *reinterpret_cast<const uint4*>(src + at.c0 * 8);
+    hi = *reinterpret_cast<const uint4*>(src + at.c1 * 8);
+  }
+  const int64_t target = p.targets[token];
+  sines(p, p.positions[token], tid, kRotaryThreads, s_cos, s_sin);
+  __syncthreads();
+  F2 co[4], si[4];
+  at.load(s_cos, s_sin, co, si);
+  turn_row<T, D, PAIRS>(p, kind, at.c0, at.c1, at.turns, co, si, lo, hi);
+  const bool stored = stored_at(p, target, tid == 0);
+  if (kind == 0 || (kind < 3 && stored)) {
+    uint16_t* out = destination<D>(p, kind, token, target, row);
+    *reinterpret_cast<uint4*>(out + at.c0 * 8) = lo;
+    *reinterpret_cast<uint4*>(out + at.c1 * 8) = hi;
+  }
+}
+
+template <typename T, int D, bool PAIRS>
+__global__ void __launch_bounds__(kRotaryThreads, kTokenCtas) rotary_tokens_kernel(const __grid_constant__ RotaryParams p) {
+  constexpr int LPR = D / 16, RPW = 32 / LPR;    // lanes of a row, rows of a warp at a time
+  __shared__ __align__(16) float s_cos[kWarps][D / 2], s_sin[kWarps][D / 2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (p.klen && blockIdx.x == 0) set_tails(p);
+  const int rows = p.hq + 2 * p.hk;
+  const Columns<PAIRS> at(p, lane % LPR);
+  for (int64_t token = int64_t(blockIdx.x) * kWarps + warp; token < p.num_tokens; token += int64_t(gridDim.x) * kWarps) {
+    const int64_t target = p.targets[token], position = p.positions[token];
+    const bool stored = stored_at(p, target, lane == 0);
+    F2 co[4], si[4];
+    for (int base = 0; base < rows; base += kBatch * RPW) {
+      uint4 raw[kBatch][2];
 #pragma unroll
-    for (int u = 0; u < R; ++u) {
-      if (__all_sync(0xffffffffu, kind[u] == 3)) break;
-      uint4 lo = raw[u][0], hi = raw[u][1];
-      if (__any_sync(0xffffffffu, kind[u] < 2)) {
-        float x[16];
-        {
-          float a[8], b[8];
-          unpack8<T>(lo, a);
-          unpack8<T>(hi, b);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = a[i], x[8 + i] = b[i];
-        }
-        if (norm) {
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sum += x[i] * x[i];
-#pragma unroll
-          for (int off = LPR / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-          const uint16_t* weight = kind[u] == 0 ? p.q_weight : kind[u] == 1 ? p.k_weight : nullptr;
-          if (weight) {
-            const float scale = rsqrtf(sum * (1.f / D) + p.eps);
-            float a[8], b[8];
-            unpack8<T>(*reinterpret_cast<const uint4*>(weight + c0 * 8), a);
-            unpack8<T>(*reinterpret_cast<const uint4*>(weight + c1 * 8), b);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] *= scale * a[i], x[8 + i] *= scale * b[i];
-          }
-        }
-        if (turns) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float& a = x[PAIRS ? 2 * i : i];
-            float& b = x[PAIRS ? 2 * i + 1 : 8 + i];
-            const float ra = a * co[i] - b * si[i];
-            b = b * co[i] + a * si[i];
-            a = ra;
-          }
-        }
-        if (kind[u] < 2) {
-          lo = make_uint4(Elem<T>::pack2(x[0], x[1]), Elem<T>::pack2(x[2], x[3]), Elem<T>::pack2(x[4], x[5]),
-                          Elem<T>::pack2(x[6], x[7]));
-          hi = make_uint4(Elem<T>::pack2(x[8], x[9]), Elem<T>::pack2(x[10], x[11]), Elem<T>::pack2(x[12], x[13]),
-                          Elem<T>::pack2(x[14], x[15]));
+      for (int u = 0; u < kBatch; ++u) {
+        const int row = base + u * RPW + lane / LPR, kind = kind_of(p, row);
+        if (kind < 3) {
+          const uint16_t* src = source(p, kind, token, row);
+          raw[u][0] = *reinterpret_cast<const uint4*>(src + at.c0 * 8);
+          raw[u][1] = *reinterpret_cast<const uint4*>(src + at.c1 * 8);
         }
       }
-      if (kind[u] == 0 || (kind[u] < 3 && stored)) {
-        uint16_t* out = dst[u] + (kind[u] == 0 ? int64_t(token) * p.hq : target) * D;
-        *reinterpret_cast<uint4*>(out + c0 * 8) = lo;
-        *reinterpret_cast<uint4*>(out + c1 * 8) = hi;
+      if (base == 0) {                           // the sines, with the first rows on their way
+        __syncwarp();                            // the last token's are read
+        sines(p, position, lane, 32, s_cos[warp], s_sin[warp]);
+        __syncwarp();
+        at.load(s_cos[warp], s_sin[warp], co, si);
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int row = base + u * RPW + lane / LPR, kind = kind_of(p, row);
+        if (__all_sync(0xffffffffu, kind == 3)) break;
+        uint4 lo = raw[u][0], hi = raw[u][1];
+        turn_row<T, D, PAIRS>(p, kind, at.c0, at.c1, at.turns, co, si, lo, hi);
+        if (kind == 0 || (kind < 3 && stored)) {
+          uint16_t* out = destination<D>(p, kind, token, target, row);
+          *reinterpret_cast<uint4*>(out + at.c0 * 8) = lo;
+          *reinterpret_cast<uint4*>(out + at.c1 * 8) = hi;
+        }
       }
     }
-    token = following;
-    if (token >= p.num_tokens) break;
   }
 }
 
@@ -213,27 +272,24 @@ bool rows16(const void* p, int64_t st, int64_t sh) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && st >= 0 && sh >= 0 && (st & 7) == 0 && (sh & 7) == 0;
 }
 
-template <typename T, int D, int R>
-void launch_rotary(const RotaryParams& p, int sms, cudaStream_t stream) {
-  constexpr int kRows = kRotaryThreads / (D / 16) * R;                 // rows of a CTA
+template <typename T, int D, bool PAIRS>
+void launch_form(const RotaryParams& p, int sms, cudaStream_t stream) {
+  constexpr int kRows = kRotaryThreads / (D / 16);
   const int batches = std::max(1, (p.hq + 2 * p.hk + kRows - 1) / kRows);
-  if (R == 1 && int64_t(p.num_tokens) * batches > int64_t(sms) * kCtas<1>) return launch_rotary<T, D, 3>(p, sms, stream);
-  // enough CTAs to fill the GPU, each with its share of the tokens
-  const dim3 grid(std::max(1, std::min(p.num_tokens, std::max(1, sms * kCtas<R> / batches))), batches);
-  if (p.interleaved)
-    rotary_append_kernel<T, D, true, R><<<grid, kRotaryThreads, 0, stream>>>(p);
+  if (int64_t(p.num_tokens) * batches <= int64_t(sms) * kRowsCtas)
+    rotary_rows_kernel<T, D, PAIRS><<<dim3(std::max(1, p.num_tokens), batches), kRotaryThreads, 0, stream>>>(p);
   else
-    rotary_append_kernel<T, D, false, R><<<grid, kRotaryThreads, 0, stream>>>(p);
+    rotary_tokens_kernel<T, D, PAIRS>
+        <<<int(std::min((int64_t(p.num_tokens) + kWarps - 1) / kWarps, int64_t(sms) * kTokenCtas)), kRotaryThreads, 0, stream>>>(p);
 }
 
 template <typename T>
 void launch_rotary(const RotaryParams& p, int head_dim, int sms, cudaStream_t stream) {
-  if (head_dim == 128)
-    launch_rotary<T, 128, 1>(p, sms, stream);
-  else if (head_dim == 64)
-    launch_rotary<T, 64, 1>(p, sms, stream);
-  else
-    launch_rotary<T, 32, 1>(p, sms, stream);
+  const auto form = p.interleaved ? (head_dim == 128 ? launch_form<T, 128, true>
+                                     : head_dim == 64 ? launch_form<T, 64, true> : launch_form<T, 32, true>)
+                                  : (head_dim == 128 ? launch_form<T, 128, false>
+                                     : head_dim == 64 ? launch_form<T, 64, false> : launch_form<T, 32, false>);
+  form(p, sms, stream);
 }
 
 }  // namespace

@@ -268,6 +268,11 @@ __device__ __forceinline__ F2 fadd2(F2 a, F2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.u) : "l"(a.u), "l"(b.u));
   return d;
 }
+__device__ __forceinline__ F2 fmul2(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.u) : "l"(a.u), "l"(b.u));
+  return d;
+}
 __device__ __forceinline__ F2 fsub2(F2 a, F2 b) {
   F2 d;
   asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d.u) : "l"(a.u), "l"(b.u));
