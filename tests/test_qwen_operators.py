@@ -152,6 +152,18 @@ def test_refusals(plain):
             decoder.beam_search(*args)
 
 
+@pytest.mark.parametrize("kind", ["dynamic", "longrope"])
+def test_frequencies_that_follow_the_length_are_refused(kind, plain):
+    model = tiny_model(32, 4, 2, torch.float32, "cpu")
+    decoder = qwen.SharedKVDecoder(model, SEQUENCES, max_new_tokens=2)
+    model.model.rotary_emb.rope_type = kind
+    for bad in (dict(rotary="fused"), dict(prefill="chunked")):
+        with pytest.raises(ValueError):
+            qwen.SharedKVDecoder(model, SEQUENCES, **bad)
+    with pytest.raises(ValueError):
+        decoder.beam_search(2)
+
+
 # ---- on the GPU ----------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(32, 4, 2), (64, 6, 2), (128, 8, 2)], ids=["d32", "d64", "d128"])

@@ -108,6 +108,8 @@ class SharedKVDecoder:
         self._slices = self._projection_slices()
         # in float32, as the embedding itself computes, whatever type the model was cast to
         self._inv_freq = model.model.rotary_emb.inv_freq.float()
+        if rotary == "fused" or prefill == "chunked":
+            self._check_frequencies()
         if prefill == "shared":
             self._prefill_shared()
         elif prefill == "chunked":
@@ -278,6 +280,13 @@ class SharedKVDecoder:
 
         return forward
 
+    def _check_frequencies(self):
+        """The fused launches read one set of frequencies: refuse an embedding whose own follow the length."""
+        kind = getattr(self.model.model.rotary_emb, "rope_type", "default")
+        if kind in ("dynamic", "longrope"):
+            raise ValueError(f"rotary positions of type {kind!r} change with the length: use rotary='model' and "
+                             "another prefill")
+
     def _rotary(self, module, q, k, v, positions, targets, status, tails):
         """q turned, k and v appended to the layer's pools, in one launch."""
         embedding = self.model.model.rotary_emb
@@ -406,6 +415,7 @@ class SharedKVDecoder:
             raise ValueError(f"the pools have room for {self.beams} beams")
         if self.generated:
             raise ValueError("beam search starts from the prompts")
+        self._check_frequencies()
         if not 0 < steps <= self.max_new_tokens:
             raise ValueError("Decode exceeds allocated max_new_tokens")
         r, dev = len(self.sequences), self.device
