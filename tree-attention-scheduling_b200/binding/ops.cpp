@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -76,6 +77,10 @@ at::Tensor rows16(const at::Tensor& x) {
   if (x.stride(2) != 1 || (x.stride(0) & 7) || (x.stride(1) & 7) || !aligned16(x))
     return x.clone(at::MemoryFormat::Contiguous);
   return x;
+}
+// An uninitialised tensor on a CUDA device (without the dispatcher's steps: these inputs need none of them).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
 }
 // Whether the memory ranges of two tensors meet.
 bool overlap(const at::Tensor& a, const at::Tensor& b) {
@@ -169,7 +174,7 @@ PyObject* rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   for (at::Tensor* w : {&qw, &kw})
     if (w->defined() && !(w->is_contiguous() && aligned16(*w))) *w = w->clone(at::MemoryFormat::Contiguous);
   if (!out.defined()) {
-    out = at::empty({n, hq, dim}, q.options());
+    out = fresh({n, hq, dim}, type, device);
   } else {
     TORCH_CHECK_VALUE(out.dim() == 3 && out.size(0) == n && out.size(1) == hq && out.size(2) == dim &&
                           out.scalar_type() == type && out.is_contiguous() && aligned16(out),
@@ -229,7 +234,7 @@ PyObject* chunk_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const c10::cuda::CUDAGuard guard(device);
   q = rows16(q), lens = packed(lens), cu = packed(cu);
   if (!out.defined()) {
-    out = at::empty({n, hq, dim}, q.options());
+    out = fresh({n, hq, dim}, type, device);
   } else {
     TORCH_CHECK_VALUE(out.dim() == 3 && out.size(0) == n && out.size(1) == hq && out.size(2) == dim &&
                           out.scalar_type() == type && out.is_contiguous() && aligned16(out),
@@ -246,7 +251,7 @@ PyObject* chunk_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                   rows = narrow(page, "page_size");
     const int64_t bytes = entry.chunk_workspace_bytes(tokens, seqs, heads, int32_t(hk), int32_t(dim), width, rows);
     at::Tensor workspace;
-    if (bytes) workspace = at::empty({bytes}, q.options().dtype(at::kByte));
+    if (bytes) workspace = fresh({bytes}, at::kByte, device);
     done(entry.chunk_attention(q.data_ptr(), q.stride(0), q.stride(1), kp.data_ptr(), vp.data_ptr(), kp.size(1),
                                table.data_ptr<int32_t>(), table.stride(0), width, rows, lens.data_ptr<int32_t>(),
                                cu.data_ptr<int32_t>(), seqs, tokens, heads, int32_t(hk), int32_t(dim), dtype_code(type),
@@ -292,13 +297,12 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       (logits.dim() == 3 && r > 1 && w > 1 && logits.stride(0) != w * logits.stride(1)))
     logits = logits.contiguous();
   const int64_t stride = logits.stride(logits.dim() == 3 && w == 1 ? 0 : logits.dim() - 2);
-  at::Tensor best = at::empty({r, k}, scores.options());
-  const at::Tensor chosen = at::empty({2, r, k}, scores.options().dtype(at::kLong));
-  at::Tensor parents = chosen.select(0, 0), tokens = chosen.select(0, 1);
+  at::Tensor best = fresh({r, k}, at::kFloat, device), parents = fresh({r, k}, at::kLong, device),
+             tokens = fresh({r, k}, at::kLong, device);
   if (r > 0) {
     const int32_t requests = narrow(r, "R"), words = narrow(vocab, "V");
     const int64_t bytes = entry.beam_workspace_bytes(requests, int32_t(w), words, int32_t(k), type);
-    const at::Tensor workspace = at::empty({bytes}, scores.options().dtype(at::kByte));
+    const at::Tensor workspace = fresh({bytes}, at::kByte, device);
     done(entry.beam_select(logits.data_ptr(), stride, scores.data_ptr<float>(), static_cast<const uint8_t*>(ptr(finished)),
                            requests, int32_t(w), words, int32_t(k), narrow(end, "end_token"), type, best.data_ptr<float>(),
                            parents.data_ptr<int64_t>(), tokens.data_ptr<int64_t>(), workspace.data_ptr(), bytes,
@@ -341,7 +345,7 @@ PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   at::DimVector shape(states.sizes().begin(), states.sizes().end());
   shape[1] = kept;
   if (!out.defined()) {
-    out = at::empty(shape, states.options());
+    out = fresh(shape, states.scalar_type(), device);
   } else {
     TORCH_CHECK_VALUE(out.sizes() == at::IntArrayRef(shape) && out.scalar_type() == states.scalar_type() && out.is_contiguous(),
                       "beam_reorder: out must be contiguous [R, K, ...] of the states' dtype");
